@@ -18,6 +18,7 @@ lib = ctypes.CDLL(LIB_PATH)
 
 DTYPE_BF16, DTYPE_F32, DTYPE_BF16X3 = 0, 1, 2
 ARCH_REFERENCE, ARCH_LLAMA = 0, 1
+KV_BF16, KV_E4M3 = 0, 1
 
 
 class Options(ctypes.Structure):
@@ -65,6 +66,42 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("dtype", c_int32), ("d_k", c_void_p), ("d_v", c_void_p), ("d_k_scale", c_void_p),
+        ("d_v_scale", c_void_p), ("page_stride", c_int64), ("n_pages", c_int32), ("page_size", c_int32),
+        ("n_kv_heads", c_int32), ("head_dim", c_int32), ("d_page_table", c_void_p), ("table_pitch", c_int32), ("pad_", c_int32),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("n_heads", c_int32), ("cache", POINTER(KvCache)), ("d_qkv", c_void_p), ("d_q", c_void_p),
+        ("ld_qkv", c_int32), ("ld_q", c_int32), ("d_cos", c_void_p), ("d_sin", c_void_p), ("n_positions", c_int32),
+        ("n_seq", c_int32), ("d_seq_start", c_void_p), ("d_pos", c_void_p), ("n_tokens", c_int32), ("pad_", c_int32),
+        ("stream", c_void_p),
+    ]
+
+
+class KvAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("n_heads", c_int32), ("cache", POINTER(KvCache)), ("d_q", c_void_p), ("d_out", c_void_p),
+        ("ld_q", c_int32), ("ld_out", c_int32), ("d_seq_start", c_void_p), ("d_pos", c_void_p), ("n_seq", c_int32),
+        ("n_tokens", c_int32), ("max_new", c_int32), ("window", c_int32), ("scale", c_float), ("pad_", c_int32),
+        ("d_workspace", c_void_p), ("workspace_bytes", c_uint64), ("stream", c_void_p),
+    ]
+
+
+class LogitRulesArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("dtype", c_int32), ("d_logits", c_void_p), ("d_out", c_void_p), ("ld_logits", c_int64),
+        ("ld_out", c_int64), ("rows", c_int32), ("vocab", c_int32), ("d_tokens", c_void_p), ("d_n_tokens", c_void_p),
+        ("d_n_prompt", c_void_p), ("ld_tokens", c_int32), ("n_masks", c_int32), ("d_mask", c_void_p), ("d_mask_row", c_void_p),
+        ("ld_mask", c_int32), ("pad_", c_int32), ("d_bias_start", c_void_p), ("d_bias_token", c_void_p), ("d_bias", c_void_p),
+        ("d_repetition", c_void_p), ("d_presence", c_void_p), ("d_frequency", c_void_p), ("stream", c_void_p),
+    ]
+
+
 # Every symbol include/ane_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "ane_device_count": (c_int32, []),
@@ -88,6 +125,10 @@ SIGNATURES = {
     "ane_op_sumsq": (c_int32, [c_void_p, c_uint64, c_float, c_void_p]),
     "ane_op_sumsq_noalloc": (c_int32, [c_void_p, c_uint64, c_float, c_void_p]),
     "ane_op_sumsq_noalloc_last_error": (c_char_p, []),
+    "ane_op_kv_append": (c_int32, [POINTER(KvAppendArgs)]),
+    "ane_op_kv_attention": (c_int32, [POINTER(KvAttentionArgs)]),
+    "ane_op_kv_attention_workspace": (c_uint64, [c_int32, c_int32, c_int32]),
+    "ane_op_logit_rules": (c_int32, [POINTER(LogitRulesArgs)]),
     "ane_dp_unique_id": (c_int32, [POINTER(c_uint8)]),
     "ane_open": (c_int32, [POINTER(Options), POINTER(c_uint16), c_uint64, POINTER(c_uint8), POINTER(c_void_p)]),
     "ane_close": (c_int32, [c_void_p]),

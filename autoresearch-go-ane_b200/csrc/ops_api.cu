@@ -15,6 +15,7 @@
 #include "engine.h"
 #include "gemm.h"
 #include "kernels.h"
+#include "serving.h"
 
 using namespace ane;
 
@@ -270,6 +271,142 @@ int32_t ane_op_gemm(const ane_gemm_args* a) {
   }
   if (rc != 0) return set_err(ANE_ERR_KERNEL, gemm_last_error());
   return 0;
+}
+
+
+}  // extern "C"
+
+// ---- serving ------------------------------------------------------------------------------------------------------
+
+// The Python binding mirrors these layouts field by field.
+static_assert(sizeof(ane_kv_cache) == 80 && sizeof(ane_kv_append_args) == 96 && sizeof(ane_kv_attention_args) == 104 &&
+                  sizeof(ane_logit_rules_args) == 160,
+              "layout of a serving structure changed: update the binding");
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// What is wrong with a cache, or nullptr.
+static const char* cache_fault(const ane_kv_cache* c, int32_t n_heads) {
+  if (!c || c->struct_size != sizeof(ane_kv_cache)) return "bad struct_size of the cache";
+  if (c->dtype != ANE_KV_BF16 && c->dtype != ANE_KV_E4M3) return "unknown dtype of the cache";
+  const bool e4m3 = c->dtype == ANE_KV_E4M3;
+  if (!kv_head_dim_supported(c->head_dim)) return "head_dim must be 32, 48, 64, 96 or 128";
+  if (c->page_size < 16 || c->page_size > 4096 || c->page_size % 16) return "page_size must be a multiple of 16 up to 4096";
+  if (c->n_pages <= 0 || c->n_kv_heads <= 0 || c->table_pitch <= 0) return "bad dimensions of the cache";
+  if (n_heads <= 0 || n_heads % c->n_kv_heads) return "n_heads must be a multiple of n_kv_heads";
+  if ((int64_t)n_heads * c->head_dim > (1 << 24) || (int64_t)c->n_kv_heads * c->head_dim > (1 << 24)) return "too many heads";
+  if (!c->d_k || !c->d_v || !c->d_page_table || (e4m3 && (!c->d_k_scale || !c->d_v_scale))) return "null pointer in the cache";
+  if (!aligned16(c->d_k) || !aligned16(c->d_v)) return "keys and values must be 16-byte aligned";
+  if (c->page_stride && (c->page_stride < (int64_t)c->n_kv_heads * c->page_size * c->head_dim || c->page_stride % (e4m3 ? 16 : 8)))
+    return "bad page_stride";
+  return nullptr;
+}
+
+static const char* batch_fault(const int32_t* start, const int32_t* pos, int32_t n_seq, int32_t n_tokens) {
+  if (!start || !pos) return "null pointer to the sequences' places";
+  if (n_seq < 0 || n_tokens < 0 || n_seq > (1 << 24)) return "bad number of sequences or tokens";
+  return nullptr;
+}
+
+// Runs one of the calls below; nothing that it throws leaves the library.
+template <class Call>
+static int32_t serve(const char* name, Call call) {
+  try {
+    const char* fault = nullptr;
+    const int32_t rc = call(&fault);
+    return fault ? set_err(rc, std::string(name) + ": " + fault) : rc;
+  } catch (...) {
+    return ANE_ERR_STATE;
+  }
+}
+
+extern "C" {
+
+int32_t ane_op_kv_append(const ane_kv_append_args* a) {
+  return serve("ane_op_kv_append", [&](const char** fault) -> int32_t {
+    if (!a || a->struct_size != sizeof(ane_kv_append_args)) return *fault = "bad struct_size", ANE_ERR_ARG;
+    if ((*fault = cache_fault(a->cache, a->n_heads))) return ANE_ERR_ARG;
+    if ((*fault = batch_fault(a->d_seq_start, a->d_pos, a->n_seq, a->n_tokens))) return ANE_ERR_ARG;
+    const ane_kv_cache& c = *a->cache;
+    if (!a->d_qkv) return *fault = "null pointer", ANE_ERR_ARG;
+    if (!aligned16(a->d_qkv) || !aligned16(a->d_q)) return *fault = "q, k and v must be 16-byte aligned", ANE_ERR_ARG;
+    if (a->ld_qkv < (a->n_heads + 2 * (int64_t)c.n_kv_heads) * c.head_dim || a->ld_qkv % 8) return *fault = "bad ld_qkv", ANE_ERR_ARG;
+    if (a->d_q && (a->ld_q < a->n_heads * c.head_dim || a->ld_q % 8)) return *fault = "bad ld_q", ANE_ERR_ARG;
+    if (a->d_q == a->d_qkv && a->ld_q != a->ld_qkv) return *fault = "in place, ld_q must be ld_qkv", ANE_ERR_ARG;
+    if (!a->d_cos != !a->d_sin) return *fault = "one of the two rotation tables is missing", ANE_ERR_ARG;
+    if (a->d_cos && (a->n_positions <= 0 || !aligned16(a->d_cos) || !aligned16(a->d_sin)))
+      return *fault = "rotation tables must be 16-byte aligned and have positions", ANE_ERR_ARG;
+    int* status = nullptr;
+    if (ensure_status(&status)) return ANE_ERR_CUDA;
+    const Batch batch = {a->d_seq_start, a->d_pos, a->n_seq, a->n_tokens};
+    const cudaError_t e = kv_append(paged_kv(c), batch, a->n_heads, reinterpret_cast<const bf16*>(a->d_qkv), a->ld_qkv,
+                                    reinterpret_cast<bf16*>(a->d_q), a->ld_q, a->d_cos, a->d_sin, a->n_positions, status,
+                                    reinterpret_cast<cudaStream_t>(a->stream));
+    return e == cudaSuccess ? 0 : cuda_fail(e, "ane_op_kv_append");
+  });
+}
+
+uint64_t ane_op_kv_attention_workspace(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim) {
+  if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || !kv_head_dim_supported(head_dim)) {
+    serve("ane_op_kv_attention_workspace", [&](const char** fault) -> int32_t { return *fault = "bad heads", ANE_ERR_ARG; });
+    return 0;
+  }
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) {
+    serve("", [&](const char**) -> int32_t { return cuda_fail(e, "ane_op_kv_attention_workspace"); });
+    return 0;
+  }
+  return kv_attention_workspace(sms, head_dim);
+}
+
+int32_t ane_op_kv_attention(const ane_kv_attention_args* a) {
+  return serve("ane_op_kv_attention", [&](const char** fault) -> int32_t {
+    if (!a || a->struct_size != sizeof(ane_kv_attention_args)) return *fault = "bad struct_size", ANE_ERR_ARG;
+    if ((*fault = cache_fault(a->cache, a->n_heads))) return ANE_ERR_ARG;
+    if ((*fault = batch_fault(a->d_seq_start, a->d_pos, a->n_seq, a->n_tokens))) return ANE_ERR_ARG;
+    const ane_kv_cache& c = *a->cache;
+    if (!a->d_q || !a->d_out || !a->d_workspace) return *fault = "null pointer", ANE_ERR_ARG;
+    if (!aligned16(a->d_q) || !aligned16(a->d_out) || !aligned16(a->d_workspace))
+      return *fault = "queries, output and workspace must be 16-byte aligned", ANE_ERR_ARG;
+    if (a->ld_q < a->n_heads * c.head_dim || a->ld_q % 8) return *fault = "bad ld_q", ANE_ERR_ARG;
+    if (a->ld_out < a->n_heads * c.head_dim || a->ld_out % 8) return *fault = "bad ld_out", ANE_ERR_ARG;
+    if (a->max_new < 1 || (int64_t)a->max_new * a->n_heads > INT32_MAX) return *fault = "bad max_new", ANE_ERR_ARG;
+    if (a->window < 0) return *fault = "bad window", ANE_ERR_ARG;
+    if (!(a->scale >= 0.f && a->scale <= 3.4e38f)) return *fault = "bad scale", ANE_ERR_ARG;
+    int* status = nullptr;
+    if (ensure_status(&status)) return ANE_ERR_CUDA;
+    const uint64_t need = ane_op_kv_attention_workspace(a->n_heads, c.n_kv_heads, c.head_dim);
+    if (!need) return ANE_ERR_CUDA;
+    if (a->workspace_bytes < need) return *fault = "workspace too small", ANE_ERR_ARG;
+    const Batch batch = {a->d_seq_start, a->d_pos, a->n_seq, a->n_tokens};
+    const cudaError_t e = kv_attention(paged_kv(c), batch, a->n_heads, reinterpret_cast<const bf16*>(a->d_q), a->ld_q,
+                                       reinterpret_cast<bf16*>(a->d_out), a->ld_out, a->max_new, a->window, a->scale, a->d_workspace,
+                                       status, reinterpret_cast<cudaStream_t>(a->stream));
+    return e == cudaSuccess ? 0 : cuda_fail(e, "ane_op_kv_attention");
+  });
+}
+
+int32_t ane_op_logit_rules(const ane_logit_rules_args* a) {
+  return serve("ane_op_logit_rules", [&](const char** fault) -> int32_t {
+    if (!a || a->struct_size != sizeof(ane_logit_rules_args)) return *fault = "bad struct_size", ANE_ERR_ARG;
+    if (a->dtype != ANE_DTYPE_F32 && a->dtype != ANE_DTYPE_BF16) return *fault = "logits must be fp32 or bf16", ANE_ERR_ARG;
+    if (!a->d_logits || !a->d_out) return *fault = "null pointer", ANE_ERR_ARG;
+    if (a->rows < 0 || a->vocab <= 0 || a->ld_logits < a->vocab || a->ld_out < a->vocab) return *fault = "bad dimensions", ANE_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(a->d_logits) % (a->dtype == ANE_DTYPE_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(a->d_out) % 4)
+      return *fault = "misaligned logits", ANE_ERR_ARG;
+    if (a->d_logits == a->d_out && (a->dtype != ANE_DTYPE_F32 || a->ld_logits != a->ld_out))
+      return *fault = "in place, logits must be fp32 with ld_out = ld_logits", ANE_ERR_ARG;
+    if (a->d_tokens && (!a->d_n_tokens || a->ld_tokens <= 0 || a->ld_tokens >= (1 << 24))) return *fault = "bad token lists", ANE_ERR_ARG;
+    if (!a->d_tokens && (a->d_repetition || a->d_presence || a->d_frequency)) return *fault = "penalties without tokens", ANE_ERR_ARG;
+    if (a->d_mask && (a->ld_mask < (a->vocab - 1) / 32 + 1 || a->n_masks < (a->d_mask_row ? 1 : a->rows))) return *fault = "bad masks", ANE_ERR_ARG;
+    if (a->d_bias_start && (!a->d_bias_token || !a->d_bias)) return *fault = "bad biases", ANE_ERR_ARG;
+    int* status = nullptr;
+    if (ensure_status(&status)) return ANE_ERR_CUDA;
+    const cudaError_t e = logit_rules(*a, status, reinterpret_cast<cudaStream_t>(a->stream));
+    return e == cudaSuccess ? 0 : cuda_fail(e, "ane_op_logit_rules");
+  });
 }
 
 }  // extern "C"

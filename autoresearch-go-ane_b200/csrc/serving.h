@@ -1,0 +1,55 @@
+// Launchers of the serving kernels (kv_append.cu, kv_attention.cu, logit_rules.cu).  Arguments have been checked by their C entry
+// points (ops_api.cu) or by the engine; each launcher returns the status of its launches.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/ane_b200.h"
+#include "common.cuh"
+
+namespace ane {
+
+// A paged cache as the kernels see it; strides in elements.
+struct PagedKv {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  long long page_stride;
+  int n_pages, page_size, kv_heads, head_dim;
+  const int* table;
+  int table_pitch;
+  bool e4m3;
+};
+PagedKv paged_kv(const ane_kv_cache& c);
+
+// The sequences of a batch: new rows [start[b], start[b + 1]) at positions pos[b]...
+struct Batch {
+  const int *start, *pos;
+  int n_seq, n_tokens;
+};
+
+bool kv_head_dim_supported(int head_dim);
+cudaError_t kv_append(const PagedKv& kv, const Batch& batch, int heads, const bf16* qkv, int ld_qkv, bf16* q, int ld_q,
+                      const float* cosb, const float* sinb, int n_positions, int* status, cudaStream_t s);
+cudaError_t kv_attention(const PagedKv& kv, const Batch& batch, int heads, const bf16* q, int ld_q, bf16* out, int ld_out,
+                         int max_new, int window, float scale, void* workspace, int* status, cudaStream_t s);
+size_t kv_attention_workspace(int sms, int head_dim);
+cudaError_t logit_rules(const ane_logit_rules_args& a, int* status, cudaStream_t s);
+
+#ifdef __CUDACC__
+// New rows and place of sequence b; none (and the status word) where its entries make no sense.
+struct Span {
+  int row, n, pos;
+};
+__device__ __forceinline__ Span span_of(const Batch& a, int b, int capacity, int most, int* status) {
+  const int row = a.start[b], end = a.start[b + 1], pos = a.pos[b];
+  if (row == end) return {row, 0, pos};
+  if (row < 0 || end < row || end > a.n_tokens || end - row > most || pos < 0 || end - row > capacity - pos) {
+    atomicCAS(status, DEV_OK, DEV_BAD_INDEX);
+    return {row, 0, pos};
+  }
+  return {row, end - row, pos};
+}
+#endif
+
+}  // namespace ane

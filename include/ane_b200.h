@@ -121,6 +121,120 @@ typedef struct ane_gemm_args {
 } ane_gemm_args;
 int32_t ane_op_gemm(const ane_gemm_args* args);
 
+/* ---- serving: paged KV cache, attention over it, rules on logits --------------
+ * What one step of a generation needs beside ane_op_gemm and ane_op_sample_rows, for sequences of different lengths.  No
+ * counterpart in the reference, which has no KV cache (ane_generate runs the three together on an engine's weights).
+ *
+ * All three only queue kernels: on the stream given (a cudaStream_t), or on the default stream for NULL.  They allocate
+ * nothing, except that the first call on a device takes its status word: make it before any stream capture.  Everything that
+ * changes from step to step (places, lengths, pages, tokens) is read on the device when the kernels run, so that a captured
+ * step can be replayed.  What the host cannot see is checked there: a page, position or row out of its range is neither read
+ * nor written, and ane_ops_device_status returns 110.  All memory belongs to the current device.
+ *
+ * A batch: the new tokens of sequence b are the rows d_seq_start[b] .. d_seq_start[b + 1] - 1 (d_seq_start has n_seq + 1
+ * entries, no order between sequences' tokens but this one; a sequence may have none), and d_pos[b] tokens are in its cache
+ * before them, so that row d_seq_start[b] + i has position d_pos[b] + i.  Rows outside all sequences stay as they are. */
+#define ANE_KV_BF16 0
+#define ANE_KV_E4M3 1 /* 8-bit floating point, a scale for each page and head: value = scale * e4m3 */
+typedef struct ane_kv_cache {
+  uint32_t struct_size;
+  int32_t dtype;             /* ANE_KV_BF16 or ANE_KV_E4M3 */
+  void* d_k;                 /* [n_pages][n_kv_heads][page_size][head_dim] */
+  void* d_v;                 /* the same; 16-byte aligned both */
+  float* d_k_scale;          /* ANE_KV_E4M3: [n_pages][n_kv_heads]; else unused */
+  float* d_v_scale;
+  int64_t page_stride;       /* elements from one page to the next (16-byte multiple); 0: n_kv_heads * page_size * head_dim */
+  int32_t n_pages;
+  int32_t page_size;         /* tokens: a multiple of 16, up to 4096 */
+  int32_t n_kv_heads;
+  int32_t head_dim;          /* 32, 48, 64, 96 or 128 */
+  const int32_t* d_page_table; /* [n_seq][table_pitch]: page of token p of sequence b at [b][p / page_size] */
+  int32_t table_pitch;       /* so a sequence has room for table_pitch * page_size tokens */
+  int32_t pad_;
+} ane_kv_cache;
+
+/* Puts the keys and values of new tokens into the cache, keys (and queries) rotated by their positions on the way: adjacent
+ * pairs (x, y) -> (x c - y s, y c + x s), the rotation of ane_step and ane_decode_greedy.  A page that is written may belong to
+ * one sequence only; full pages may be shared.
+ *
+ * ANE_KV_E4M3: the scale of a page and head is the smallest power of two, at least 2^-126, by which its largest value fits 448;
+ * the call that writes a page's first token sets it anew, later calls let it grow, and the tokens that the page holds already
+ * are rounded again to the larger scale (powers of two: only values that become subnormal, below 2^-13 of the page's largest, lose bits).
+ * Infinities are stored as the largest value, NaN as NaN; neither counts for the scale. */
+typedef struct ane_kv_append_args {
+  uint32_t struct_size;
+  int32_t n_heads;           /* query heads, a multiple of n_kv_heads */
+  const ane_kv_cache* cache;
+  const void* d_qkv;         /* bf16 [n_tokens][ld_qkv]: q | k | v of a token, as ane_step's QKV product has them */
+  void* d_q;                 /* bf16 [n_tokens][ld_q]: rotated queries; may be d_qkv (ld_q = ld_qkv); NULL: not wanted */
+  int32_t ld_qkv, ld_q;      /* multiples of 8 */
+  const float* d_cos;        /* [n_positions][head_dim / 2]; both NULL: no rotation */
+  const float* d_sin;
+  int32_t n_positions;
+  int32_t n_seq;
+  const int32_t* d_seq_start;
+  const int32_t* d_pos;
+  int32_t n_tokens;          /* rows of d_qkv and d_q */
+  int32_t pad_;
+  void* stream;
+} ane_kv_append_args;
+int32_t ane_op_kv_append(const ane_kv_append_args* args);
+
+/* Attention of new tokens over their sequences' caches, the new tokens' own keys included (append first): the token at
+ * position p sees positions 0 .. p, with a window only the last `window` of them.  One token a sequence or many.  Softmax statistics
+ * and sums in fp32, probabilities enter their product in 16 bits.  Results are the same from call to call. */
+typedef struct ane_kv_attention_args {
+  uint32_t struct_size;
+  int32_t n_heads;
+  const ane_kv_cache* cache;
+  const void* d_q;           /* bf16 [n_tokens][ld_q], n_heads * head_dim columns, rotated */
+  void* d_out;               /* bf16 [n_tokens][ld_out] */
+  int32_t ld_q, ld_out;      /* multiples of 8 */
+  const int32_t* d_seq_start;
+  const int32_t* d_pos;
+  int32_t n_seq;
+  int32_t n_tokens;
+  int32_t max_new;           /* no sequence has more new tokens than this */
+  int32_t window;            /* 0: all positions */
+  float scale;               /* of the scores; 0: head_dim^-1/2 */
+  int32_t pad_;
+  void* d_workspace;         /* 16-byte aligned; for one call at a time, its content does not matter */
+  uint64_t workspace_bytes;  /* at least ane_op_kv_attention_workspace() */
+  void* stream;
+} ane_kv_attention_args;
+int32_t ane_op_kv_attention(const ane_kv_attention_args* args);
+/* Bytes that suffice on the current device for any batch and lengths; 0: an error. */
+uint64_t ane_op_kv_attention_workspace(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+
+/* Penalties, biases and grammar masks on rows of logits, in this order, each rounded to fp32.  With n = how often token v is among the
+ * row's output tokens:  v among the row's prompt or output tokens: x > 0 ? x / repetition : x * repetition;  x -= frequency * n;
+ * n > 0: x -= presence;  x += the row's bias for v;  v not allowed by the row's mask: x = -infinity, whatever x is. */
+typedef struct ane_logit_rules_args {
+  uint32_t struct_size;
+  int32_t dtype;             /* of d_logits: ANE_DTYPE_F32 or ANE_DTYPE_BF16 */
+  const void* d_logits;      /* [rows][ld_logits] */
+  float* d_out;              /* [rows][ld_out]; may be d_logits (fp32, ld_out = ld_logits) */
+  int64_t ld_logits, ld_out;
+  int32_t rows, vocab;
+  const int32_t* d_tokens;   /* [rows][ld_tokens]; ids outside the vocabulary are passed over; NULL: no penalties */
+  const int32_t* d_n_tokens; /* [rows]: tokens of a row that count, its prompt's and its output's */
+  const int32_t* d_n_prompt; /* [rows]: how many of them, from the first, are the prompt's; NULL: none */
+  int32_t ld_tokens;         /* below 2^24 */
+  int32_t n_masks;
+  const uint32_t* d_mask;    /* [n_masks][ld_mask]: bit v % 32 of word v / 32 allows token v; NULL: no masks */
+  const int32_t* d_mask_row; /* [rows]: a row's mask, negative: none; NULL: row r has mask r */
+  int32_t ld_mask;           /* words */
+  int32_t pad_;
+  const int32_t* d_bias_start; /* [rows + 1]: row r has entries d_bias_start[r] .. d_bias_start[r + 1] - 1; NULL: no biases */
+  const int32_t* d_bias_token; /* ids outside the vocabulary are passed over; the last entry of a token counts; up to 65535 a row */
+  const float* d_bias;
+  const float* d_repetition; /* [rows] each; NULL: none */
+  const float* d_presence;
+  const float* d_frequency;
+  void* stream;
+} ane_logit_rules_args;
+int32_t ane_op_logit_rules(const ane_logit_rules_args* args);
+
 
 /* ============================================================================
  * Engine: the drop-in surface behind ane.Engine (ane/engine.go).
