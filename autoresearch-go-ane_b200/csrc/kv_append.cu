@@ -20,7 +20,7 @@ PagedKv paged_kv(const ane_kv_cache& c) {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kTokens = 8;  // tokens of a block that rotates rows
+constexpr int kEach = 4;  // groups of eight elements that a thread rotates
 
 struct Append {
   PagedKv kv;
@@ -92,21 +92,26 @@ __device__ __forceinline__ void store_eight(bf16* p, const Eight& e) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows of up to kTokens tokens: the queries of all caches, keys and values too of a bf16 one.
+// kEach * kThreads groups of eight elements of the tokens' rows, in the order of memory: the queries of all caches, keys and values too of a
+// bf16 one.
 __device__ __forceinline__ void append_rows(const Append& a, int block) {
-  const int first = block * kTokens, tid = threadIdx.x;
+  const int tid = threadIdx.x;
   const int hd = a.kv.head_dim, half = hd >> 1, page = a.kv.page_size;
   const int capacity = (int)min((long long)a.kv.table_pitch * page, (long long)INT32_MAX);
+  const int q_vec = a.q ? a.heads * hd / 8 : 0, kv_vec = a.kv.e4m3 ? 0 : a.kv.kv_heads * hd / 8, vec = q_vec + 2 * kv_vec;
+  const long long begin = (long long)block * (kEach * kThreads);
+  const int first = (int)(begin / vec), v0 = (int)(begin - (long long)first * vec);
   // the sequence of the block's first row; the next ones are found from there
-  int b0 = count_before<kThreads>(a.batch.n_seq, tid, [&](int i) { return a.batch.start[i + 1] <= first; });
-  const int q_vec = a.q ? a.heads * hd / 8 : 0, kv_vec = a.kv.e4m3 ? 0 : a.kv.kv_heads * hd / 8;
-  const int vec = q_vec + 2 * kv_vec, last = min(first + kTokens, a.batch.n_tokens);
-  for (int i = tid; i < (last - first) * vec; i += kThreads) {
-    const int row = first + i / vec, v = i % vec;
-    int b = b0;
+  int b = count_before<kThreads>(a.batch.n_seq, tid, [&](int i) { return a.batch.start[i + 1] <= first; });
+  Span s = {0, 0, 0};
+  int known = -1;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int u = v0 + tid + i * kThreads, row = first + u / vec, v = u % vec;
+    if (row >= a.batch.n_tokens) break;
     while (b < a.batch.n_seq && a.batch.start[b + 1] <= row) ++b;
-    if (b == a.batch.n_seq) continue;
-    const Span s = span_of(a.batch, b, capacity, INT32_MAX, a.status);
+    if (b == a.batch.n_seq) break;
+    if (b != known) s = span_of(a.batch, known = b, capacity, INT32_MAX, a.status);
     if (s.n == 0 || row < s.row) continue;
     const int pos = s.pos + row - s.row;
     const int part = v < q_vec ? 0 : v < q_vec + kv_vec ? 1 : 2;
@@ -117,19 +122,20 @@ __device__ __forceinline__ void append_rows(const Append& a, int block) {
       continue;
     }
     const int in_col = col + (part == 0 ? 0 : (a.heads + (part - 1) * a.kv.kv_heads) * hd);
-    const size_t at = (size_t)pos * half + (col % hd >> 1);
+    const int head = col / hd, in_head = col - head * hd;
+    const size_t at = (size_t)pos * half + (in_head >> 1);
     const Eight e = load_eight(a.qkv + (size_t)row * a.ld_qkv + in_col, turn ? a.cosb + at : nullptr, turn ? a.sinb + at : nullptr);
     if (part == 0) {
       store_eight(a.q + (size_t)row * a.ld_q + col, e);
       continue;
     }
-    const int p = a.kv.table[(size_t)b * a.kv.table_pitch + pos / page];
+    const int slot = pos / page, p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
     if (p < 0 || p >= a.kv.n_pages) {
       atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
       continue;
     }
     bf16* cache = reinterpret_cast<bf16*>(part == 1 ? a.kv.k : a.kv.v);
-    store_eight(cache + p * a.kv.page_stride + ((size_t)(col / hd) * page + pos % page) * hd + col % hd, e);
+    store_eight(cache + p * a.kv.page_stride + ((size_t)head * page + pos - slot * page) * hd + in_head, e);
   }
 }
 
@@ -256,7 +262,9 @@ cudaError_t kv_append(const PagedKv& kv, const Batch& batch, int heads, const bf
                       const float* cosb, const float* sinb, int n_positions, int* status, cudaStream_t s) {
   if (batch.n_seq == 0 || batch.n_tokens == 0) return cudaSuccess;
   Append a = {kv, batch, qkv, q, cosb, sinb, ld_qkv, ld_q, heads, n_positions, 0, 0, status};
-  if (q || !kv.e4m3) a.rows_blocks = (batch.n_tokens + kTokens - 1) / kTokens;
+  const long long vec = (long long)batch.n_tokens * ((q ? heads : 0) + (kv.e4m3 ? 0 : 2 * kv.kv_heads)) * kv.head_dim / 8;
+  if ((vec + kEach * kThreads - 1) / (kEach * kThreads) > INT32_MAX) return cudaErrorInvalidValue;
+  a.rows_blocks = (int)((vec + kEach * kThreads - 1) / (kEach * kThreads));
   long long tasks = 0;
   if (kv.e4m3) {
     a.units = batch.n_tokens / kv.page_size + 2 * batch.n_seq;

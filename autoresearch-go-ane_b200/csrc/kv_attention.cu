@@ -1,12 +1,12 @@
 // Attention of new tokens over a paged KV cache (ane_op_kv_attention).
 //
 // The query heads of a KV head share its keys, so they are rows of one product: row r of a KV head's queries is token r / group,
-// head r % group, and 16 rows (m16n8k16 on mma.sync) are a tile.  Single tokens fill a tile badly, but they are bound by
-// the bytes of the cache, and the products take a fraction of the time that their operands need to arrive.
+// head r % group.  Products are m16n8k16 on mma.sync: single tokens are bound by the bytes of the cache, and their
+// products take a fraction of the time that the operands need to arrive.
 //
-//   few rows (kM = 1): a CTA holds one tile of 16 rows; its four warps take 16 of every 64 keys each, with softmax statistics of
-//     their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
-//   many rows (kM = 4): a CTA holds 64 rows, a warp 16 of them, and all warps go over all keys.
+//   few rows (up to 16 a KV head): a CTA holds 8 or 16 rows; its four warps take 16 of every 64 keys each, with softmax statistics
+//     of their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
+//   many rows: a CTA holds 64 or 128 rows, a warp a quarter of them, and all warps go over all keys.
 //
 // Keys and values come by cp.async into a ring of stages of 64 keys.  8-bit ones stay 8-bit until they are in registers, where they
 // become f16, which holds e4m3 exactly: queries are brought to f16 by a power of two per row, scales of keys go onto the
@@ -47,7 +47,6 @@ struct Layout {
   static constexpr int RB = HD * ES, GB = kGroup * RB, CPR = RB / 16;  // bytes of a row, of 16 rows; 16-byte pieces of a row
   static constexpr int VK = RB % 64 == 0 ? 16 : RB % 32 == 0 ? 8 : 4;   // bytes that a thread loads of K rows at a time
   static constexpr int VV = RB % 128 == 0 ? 16 : RB % 64 == 0 ? 8 : RB % 32 == 0 ? 4 : 2;  // of V rows
-  static constexpr int STAGES = GB * 2 * kWarps * 4 <= 65536 ? 4 : 3;
   static constexpr int STAGE = kWarps * 2 * GB;
 };
 
@@ -227,37 +226,36 @@ __device__ Plan make_plan(const Attn& a, int capacity) {
   return p;
 }
 
-// ---- the products of 16 keys and 16 rows ------------------------------------------------------------------------------------------
-template <int HD, bool F8>
-struct Rows {  // a warp's 16 rows: queries as left operands, output, statistics of rows g and g + 8
-  uint32_t q[HD / 16][4];
-  float o[HD / 8][4];
-  float m[2], l[2], mult[2];  // mult: what brings a row's products to scores in log2
-  int pos[2];                 // positions of the two rows; -1: no such row
-  float v_ref;                // 8 bits: o is in units of this times 1 / kPScale
+// ---- the products of 16 keys and a warp's rows ----------------------------------------------------------------------------------
+// Scores as K q^T and outputs as V^T p^T: keys, and then columns of the output, are the 16 rows of a product, queries its 8 columns, so
+// that a group of up to 8 heads takes half of the products, registers and softmax arithmetic of the other way round.
+template <int HD, bool F8, int NB>
+struct Rows {  // 8 * NB rows of queries
+  uint32_t q[NB][HD / 16][2];  // right operands: the thread's row g of each eight
+  float o[NB][HD / 16][4];     // columns of the output column(2 y, g) and column(2 y + 1, g), for rows 2 j and 2 j + 1
+  float m[NB][2], l[NB][2], mult[NB][2];  // rows 2 j and 2 j + 1; mult: what brings products to scores in log2
+  int pos[NB][2];                         // their positions; -1: no such row
+  float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = kPScale / v_ref
 };
 
-template <int HD, bool F8>
-__device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int rows0, int head, Rows<HD, F8>& r) {
+template <int HD, bool F8, int NB>
+__device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int rows0, int head, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
   const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, n_rows = s.n * a.group;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int row = rows0 + g + 8 * h;
+  for (int n = 0; n < NB; ++n) {
+    const int row = rows0 + 8 * n + g;
     const bool there = row < n_rows;
     const int t = there ? row / a.group : 0, hd = there ? row - t * a.group : 0;
-    r.pos[h] = there ? s.pos + t : -1;
-    r.m[h] = -INFINITY;
-    r.l[h] = 0.f;
-    r.mult[h] = a.scale_log2;
     const bf16* q = a.q + (size_t)(s.row + t) * a.ld_q + (size_t)(head * a.group + hd) * HD;
+    float mult = a.scale_log2;
     if (F8) {
       uint2 w[HD / 16];
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
         // word i of the thread's bytes of a K row: four elements
-        const int at = L::VK / 4 * j * 4 + (i / (L::VK / 4)) * 4 * L::VK + (i % (L::VK / 4)) * 4;
+        const int at = L::VK * j + i / (L::VK / 4) * 4 * L::VK + i % (L::VK / 4) * 4;
         w[i] = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
         top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(w[i].x << 16)), fabsf(__uint_as_float(w[i].x & 0xffff0000u))),
                                fmaxf(fabsf(__uint_as_float(w[i].y << 16)), fabsf(__uint_as_float(w[i].y & 0xffff0000u)))));
@@ -268,11 +266,11 @@ __device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int r
       const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);
       const bool fine = top > 0.f && top < INFINITY;
       const float by = fine ? __uint_as_float((uint32_t)min(254 + 8 - e, 254) << 23) : 1.f;
-      r.mult[h] = a.scale_log2 / by;
+      mult /= by;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        r.q[i][h] = pack<true>(__uint_as_float(w[i].x << 16) * by, __uint_as_float(w[i].x & 0xffff0000u) * by);
-        r.q[i][2 + h] = pack<true>(__uint_as_float(w[i].y << 16) * by, __uint_as_float(w[i].y & 0xffff0000u) * by);
+        r.q[n][i][0] = pack<true>(__uint_as_float(w[i].x << 16) * by, __uint_as_float(w[i].x & 0xffff0000u) * by);
+        r.q[n][i][1] = pack<true>(__uint_as_float(w[i].y << 16) * by, __uint_as_float(w[i].y & 0xffff0000u) * by);
       }
     } else {
 #pragma unroll
@@ -280,154 +278,164 @@ __device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int r
         // words 2 i and 2 i + 1 of the thread's bytes of a K row
         const int word = 2 * i, at = (L::VK * j + word / (L::VK / 4) * 4 * L::VK + word % (L::VK / 4) * 4) / 2;
         const uint2 w = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
-        r.q[i][h] = w.x;
-        r.q[i][2 + h] = w.y;
+        r.q[n][i][0] = w.x;
+        r.q[n][i][1] = w.y;
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.f;
+    for (int h = 0; h < 2; ++h) {
+      const int mine = rows0 + 8 * n + 2 * j + h;
+      r.pos[n][h] = mine < n_rows ? s.pos + mine / a.group : -1;
+      r.m[n][h] = -INFINITY;
+      r.l[n][h] = 0.f;
+      r.mult[n][h] = F8 ? __shfl_sync(0xffffffffu, mult, (2 * j + h) * 4) : mult;
+    }
+#pragma unroll
+    for (int y = 0; y < HD / 16; ++y) r.o[n][y][0] = r.o[n][y][1] = r.o[n][y][2] = r.o[n][y][3] = 0.f;
+  }
   r.v_ref = kLowest;
+  r.v_inv = kPScale / kLowest;
 }
 
-// Whether the exponent of a 16-bit value of a pair is all ones.
+// Whether one of a word's values is infinite or NaN.
 template <bool F8>
 __device__ __forceinline__ bool not_finite(uint32_t w) {
-  const uint32_t e = F8 ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || (w >> 16 & e) == e;
+  if (F8) return (w & 0x7fu) == 0x7fu || (w >> 8 & 0x7fu) == 0x7fu || (w >> 16 & 0x7fu) == 0x7fu || (w >> 24 & 0x7fu) == 0x7fu;
+  return (w & 0x7f80u) == 0x7f80u || (w >> 16 & 0x7f80u) == 0x7f80u;
 }
 
-// Column of the output that element i of register pair x (n-tile x, column 2 j + i) stands for.
+// Column of the output that group x of a thread's bytes of V rows (element x) stands for in the threads with this g.
 template <int HD, bool F8>
-__device__ __forceinline__ int column(int x, int j, int i) {
+__device__ __forceinline__ int column(int x, int g) {
   using L = Layout<HD, F8>;
   constexpr int EV = L::VV / L::ES;
-  return x / EV * 8 * EV + (2 * j + i) * EV + x % EV;
+  return x / EV * 8 * EV + g * EV + x % EV;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 matrix of 16-bit values
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
 }
 
 // 16 keys at positions key0.. against the warp's rows.  `checked`: some row does not see some key.
-template <int HD, bool F8>
+template <int HD, bool F8, int NB>
 __device__ __forceinline__ void keys_16(const char* ks, const char* vs, int key0, bool checked, int window, float k_scale,
-                                        float v_scale, Rows<HD, F8>& r) {
+                                        float v_scale, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
   const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  float s[2][4];
+  float s[NB][4];  // keys g (0, 1) and g + 8 (2, 3), rows 2 j and 2 j + 1
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-    uint32_t w[L::RB / 16];
-    const int row = t * 8 + g;
+  for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
-      const int byte = L::VK * j + 4 * L::VK * i;
-      lds<L::VK>(ks + piece<L::CPR, false>(row, byte >> 4) * 16 + (byte & 15), w + i * (L::VK / 4));
-    }
+  for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
+    const int byte = L::VK * j + 4 * L::VK * i;
+    uint32_t u[L::VK / 4], w[L::VK / 4];  // of keys g and g + 8
+    lds<L::VK>(ks + piece<L::CPR, false>(g, byte >> 4) * 16 + (byte & 15), u);
+    lds<L::VK>(ks + piece<L::CPR, false>(8 + g, byte >> 4) * 16 + (byte & 15), w);
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-      if (F8) mma<true>(s[t], r.q[i], e4m3_to_f16(w[i]), e4m3_to_f16(w[i] >> 16));
-      else mma<false>(s[t], r.q[i], w[2 * i], w[2 * i + 1]);
+    for (int x = 0; x < L::VK / 4; x += F8 ? 1 : 2) {
+      const uint32_t k[4] = {F8 ? e4m3_to_f16(u[x]) : u[x], F8 ? e4m3_to_f16(w[x]) : w[x], F8 ? e4m3_to_f16(u[x] >> 16) : u[x + !F8],
+                             F8 ? e4m3_to_f16(w[x] >> 16) : w[x + !F8]};
+      const int step = F8 ? i * (L::VK / 4) + x : (i * (L::VK / 4) + x) / 2;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma<F8>(s[n], k, r.q[n][step][0], r.q[n][step][1]);
     }
   }
-  uint32_t seen = 0xffu;  // bit 4 t + i of s[t][i]
+  uint32_t seen = 0xffffffffu;  // bit 4 n + i of s[n][i]
+  if (checked) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[t][i] *= r.mult[i >> 1] * (F8 ? k_scale : 1.f);
-      if (checked) {
-        const int key = key0 + t * 8 + 2 * j + (i & 1), pos = r.pos[i >> 1];
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + g + 8 * (i >> 1), pos = r.pos[n][i & 1];
         if (key > pos || (window && key <= pos - window)) {
-          s[t][i] = -INFINITY;
-          seen &= ~(1u << (4 * t + i));
+          s[n][i] = -INFINITY;
+          seen &= ~(1u << (4 * n + i));
         }
       }
-    }
-  float fix[2] = {1.f, 1.f}, base[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    top = fmaxf(top, r.m[h]);
-    base[h] = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2 of -infinity, which is 0
-    fix[h] = exp2_fast(r.m[h] - base[h]);
-    r.m[h] = top;
   }
   float into = 1.f;
   if (F8) {
-    if (v_scale > r.v_ref) {
+    if (v_scale > r.v_ref) {  // statistics keep their unit, the output changes to the new one
       const float by = r.v_ref / v_scale;
       r.v_ref = v_scale;
-      // statistics keep their unit, the output changes to the new one
+      r.v_inv = kPScale / v_scale;
 #pragma unroll
-      for (int x = 0; x < HD / 8; ++x)
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.o[x][i] *= by;
+        for (int y = 0; y < HD / 16; ++y)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r.o[n][y][i] *= by;
     }
-    into = v_scale / r.v_ref * kPScale;
+    into = v_scale * r.v_inv;
   }
-  float sum[2] = {0.f, 0.f};
+  uint32_t p[NB][2];
+  bool moved = false;
+  float fix[NB][2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int n = 0; n < NB; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[t][i] = exp2_fast(s[t][i] - base[i >> 1]);
-      sum[i >> 1] += s[t][i];
-      if (F8) s[t][i] *= into;
+    for (int h = 0; h < 2; ++h) {
+      const float mult = F8 ? fmaxf(r.mult[n][h] * k_scale, kLowest) : r.mult[n][h];  // not 0, so that hidden scores stay -infinity
+      float top = fmaxf(s[n][h], s[n][2 + h]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      top = fmaxf(top * mult, r.m[n][h]);
+      const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2 of -infinity, which is 0
+      fix[n][h] = exp2_fast(r.m[n][h] - base);
+      moved |= r.m[n][h] != top;
+      r.m[n][h] = top;
+      s[n][h] = exp2_fast(fmaf(s[n][h], mult, -base));
+      s[n][2 + h] = exp2_fast(fmaf(s[n][2 + h], mult, -base));
+      r.l[n][h] = fmaf(r.l[n][h], fix[n][h], s[n][h] + s[n][2 + h]);  // the thread's own keys; joined at the end
+      if (F8) {
+        s[n][h] *= into;
+        s[n][2 + h] *= into;
+      }
     }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) r.l[h] = r.l[h] * fix[h] + sum[h];  // the thread's own keys; joined at the end
-  if (__any_sync(0xffffffffu, fix[0] != 1.f || fix[1] != 1.f)) {
-#pragma unroll
-    for (int x = 0; x < HD / 8; ++x) {
-      r.o[x][0] *= fix[0];
-      r.o[x][1] *= fix[0];
-      r.o[x][2] *= fix[1];
-      r.o[x][3] *= fix[1];
-    }
+    // probabilities in 16 bits: their rounding is half a step of the output's own type or less
+    p[n][0] = transposed(pack<F8>(s[n][0], s[n][1]));
+    p[n][1] = transposed(pack<F8>(s[n][2], s[n][3]));
   }
-  // probabilities in 16 bits: their rounding is half a step of the output's own type or less
-  const uint32_t p[4] = {pack<F8>(s[0][0], s[0][1]), pack<F8>(s[0][2], s[0][3]), pack<F8>(s[1][0], s[1][1]),
-                         pack<F8>(s[1][2], s[1][3])};
-  constexpr int EV = L::VV / L::ES, WV = L::VV >= 4 ? L::VV / 4 : 1;
+  if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int y = 0; y < HD / 16; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.o[n][y][i] *= fix[n][i & 1];
+  }
   bool odd = false;
   if (checked) {
     // a value that is infinite or NaN must not reach rows that do not see its key, and 0 * NaN is NaN
 #pragma unroll 1
-    for (int i = lane; i < L::GB / 4; i += 32) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(vs + 4 * i);
-      if (F8) odd |= (w & 0x7fu) == 0x7fu || (w >> 8 & 0x7fu) == 0x7fu || (w >> 16 & 0x7fu) == 0x7fu || (w >> 24 & 0x7fu) == 0x7fu;
-      else odd |= not_finite<false>(w);
-    }
+    for (int i = lane; i < L::GB / 4; i += 32) odd |= not_finite<F8>(*reinterpret_cast<const uint32_t*>(vs + 4 * i));
     odd = __any_sync(0xffffffffu, odd);
   }
   if (odd) {
     // one product after the other, unseen ones left out
 #pragma unroll 1
     for (int k = 0; k < kGroup; ++k) {
-      const int from = (lane & ~3) | (k & 7) >> 1, i = k & 1;
-      float w[2];
-      bool see[2];
+      const int from = (k & 7) * 4 + j;
+      const uint32_t see = __shfl_sync(0xffffffffu, seen, from) >> (k < 8 ? 0 : 2);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float lo = k < 8 ? s[0][2 * h] : s[1][2 * h], hi = k < 8 ? s[0][2 * h + 1] : s[1][2 * h + 1];
-        w[h] = __shfl_sync(0xffffffffu, i ? hi : lo, from);
-        see[h] = __shfl_sync(0xffffffffu, seen >> (4 * (k >> 3) + 2 * h + i) & 1u, from) != 0;
-      }
+      for (int n = 0; n < NB; ++n) {
+        const float w0 = __shfl_sync(0xffffffffu, k < 8 ? s[n][0] : s[n][2], from), w1 = __shfl_sync(0xffffffffu, k < 8 ? s[n][1] : s[n][3], from);
 #pragma unroll
-      for (int x = 0; x < HD / 8; ++x)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int byte = column<HD, F8>(x, j, c) * L::ES;
+        for (int x = 0; x < HD / 8; ++x) {
+          const int byte = column<HD, F8>(x, g) * L::ES;
           const char* at = vs + piece<L::CPR, true>(k, byte >> 4) * 16 + (byte & 15);
           const float v = F8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*reinterpret_cast<const unsigned char*>(at), __NV_E4M3)))
                              : __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(at) << 16);
-          if (see[0]) r.o[x][c] += w[0] * v;
-          if (see[1]) r.o[x][2 + c] += w[1] * v;
+          if (see >> (4 * n) & 1u) r.o[n][x >> 1][2 * (x & 1)] += w0 * v;
+          if (see >> (4 * n + 1) & 1u) r.o[n][x >> 1][2 * (x & 1) + 1] += w1 * v;
         }
+      }
     }
     return;
   }
+  constexpr int EV = L::VV / L::ES, WV = L::VV >= 4 ? L::VV / 4 : 1;
 #pragma unroll
   for (int i = 0; i < L::RB / (8 * L::VV); ++i) {
     const int byte = L::VV * g + 8 * L::VV * i;
@@ -439,39 +447,58 @@ __device__ __forceinline__ void keys_16(const char* ks, const char* vs, int key0
     }
 #pragma unroll
     for (int x = 0; x < WV; ++x) {
-      const uint32_t b0 = F8 ? __byte_perm(w[0][x], w[1][x], 0x5140) : __byte_perm(w[0][x], w[1][x], 0x5410);
-      const uint32_t b1 = F8 ? __byte_perm(w[2][x], w[3][x], 0x5140) : __byte_perm(w[2][x], w[3][x], 0x5410);
       if (F8) {
-        const int n = i * EV + 4 * x;
-        mma<true>(r.o[n], p, e4m3_to_f16(b0), e4m3_to_f16(b1));
-        mma<true>(r.o[n + 1], p, e4m3_to_f16(b0 >> 16), e4m3_to_f16(b1 >> 16));
+        // two columns of two keys in a word: (key, key + 1) of one column, then of the next
+        const uint32_t b0 = __byte_perm(w[0][x], w[1][x], 0x5140), b1 = __byte_perm(w[2][x], w[3][x], 0x5140);
+        const uint32_t v[4] = {e4m3_to_f16(b0), e4m3_to_f16(b0 >> 16), e4m3_to_f16(b1), e4m3_to_f16(b1 >> 16)};
+        const int y = (i * EV + 4 * x) / 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y], v, p[n][0], p[n][1]);
         if (EV > 2) {
           const uint32_t c0 = __byte_perm(w[0][x], w[1][x], 0x7362), c1 = __byte_perm(w[2][x], w[3][x], 0x7362);
-          mma<true>(r.o[n + 2], p, e4m3_to_f16(c0), e4m3_to_f16(c1));
-          mma<true>(r.o[n + 3], p, e4m3_to_f16(c0 >> 16), e4m3_to_f16(c1 >> 16));
+          const uint32_t u[4] = {e4m3_to_f16(c0), e4m3_to_f16(c0 >> 16), e4m3_to_f16(c1), e4m3_to_f16(c1 >> 16)};
+#pragma unroll
+          for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y + 1], u, p[n][0], p[n][1]);
         }
       } else {
-        const int n = i * EV + 2 * x;
-        mma<false>(r.o[n], p, b0, b1);
-        mma<false>(r.o[n + 1], p, __byte_perm(w[0][x], w[1][x], 0x7632), __byte_perm(w[2][x], w[3][x], 0x7632));
+        const uint32_t v[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
+                               __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
+        const int y = (i * EV + 2 * x) / 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[n][0], p[n][1]);
       }
     }
   }
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------------------
-template <int HD, bool F8, int kM>
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
+// kSplit: the four warps share 8 * NB rows and take 16 of every 64 keys each; otherwise each has 8 * NB rows and takes all keys.
+template <int HD, bool F8, int NB, bool kSplit>
+struct Form {
   using L = Layout<HD, F8>;
-  constexpr int kRows = 16 * kM;
+  static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
+  // resident CTAs wanted: registers for outputs and queries decide
+  static constexpr int kRegs = NB * (HD / 16 * 6 + 16);
+  static constexpr int kCtas = kRegs <= 80 ? 4 : kRegs <= 112 ? 3 : 2;
+  static constexpr int kRoom = 224 * 1024 / kCtas - 4096, kFit = kRoom / L::STAGE;
+  static constexpr int kStages = kFit < 3 ? 3 : kFit > 6 ? 6 : kFit;
+  static constexpr int kJoin = kSplit ? kWarps * kRows * HD * 4 : 0;
+  static constexpr int kSmem = kStages * L::STAGE > kJoin ? kStages * L::STAGE : kJoin;
+};
+
+template <int HD, bool F8, int NB, bool kSplit>
+__global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_attention_kernel(const Attn a) {
+  using L = Layout<HD, F8>;
+  using F = Form<HD, F8, NB, kSplit>;
+  constexpr int kRows = F::kRows, kStages = F::kStages;
   extern __shared__ __align__(128) char ring[];
-  __shared__ float scales[L::STAGES][kWarps][2];
-  __shared__ float join_m[kWarps][16], join_l[kWarps][16];
+  __shared__ float2 scales[kStages][kWarps];
+  __shared__ float join_m[kWarps][8 * NB], join_l[kWarps][8 * NB];
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
   const int page = a.kv.page_size;
   const int capacity = (int)min((long long)a.kv.table_pitch * page, (long long)INT32_MAX);
-  Plan plan = make_plan<kRows>(a, capacity);
+  const Plan plan = make_plan<kRows>(a, capacity);
   if (tid == 0) a.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
   const uint32_t ring_at = smem_u32(ring);
   int b = plan.b, mt = plan.mt, head = plan.head, off = plan.off;
@@ -487,19 +514,20 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
     const int count = plan.whole ? tiles : (int)min((long long)(tiles - off), plan.last - unit);
     const int tile0 = range.t0() + off;
 
-    // copies of tile0 + i, i < count: this warp's 16 keys of each.  Page numbers and scales of 32 tiles ahead are in its lanes.
-    int my_page = -1;
+    // copies of tile0 + i, i < count: this warp's 16 keys of each.  Where they lie (in 16-byte pieces; all ones: nowhere) and their scales,
+    // of 32 tiles ahead, are in its lanes.
+    uint32_t my_at = 0xffffffffu;
     float my_k = 1.f, my_v = 1.f;
     auto look_up = [&](int i) {
       const int key = (tile0 + i + lane) * kTile + warp * kGroup;
-      my_page = -1;
+      my_at = 0xffffffffu;
       my_k = my_v = 1.f;
       if (i + lane < count && key < range.hi && key + kGroup > range.lo) {
-        const int p = a.kv.table[(size_t)b * a.kv.table_pitch + key / page];
+        const int slot = key / page, p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
         if (p < 0 || p >= a.kv.n_pages) {
           atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
         } else {
-          my_page = p;
+          my_at = (uint32_t)(((unsigned long long)p * a.kv.page_stride + ((size_t)head * page + key - slot * page) * HD) * L::ES >> 4);
           if (F8) {
             my_k = a.kv.k_scale[(size_t)p * a.kv.kv_heads + head];
             my_v = a.kv.v_scale[(size_t)p * a.kv.kv_heads + head];
@@ -507,61 +535,69 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
         }
       }
     };
+    int to_stage = 0, from_stage = 0;
     auto copy = [&](int i) {
       if (i < count) {
         if ((i & 31) == 0) look_up(i);
-        const int p = __shfl_sync(0xffffffffu, my_page, i & 31);
-        const int key0 = (tile0 + i) * kTile + warp * kGroup, stage = i % L::STAGES;
+        const uint32_t at = __shfl_sync(0xffffffffu, my_at, i & 31);
+        const int key0 = (tile0 + i) * kTile + warp * kGroup;
         if (F8) {
           const float ks = __shfl_sync(0xffffffffu, my_k, i & 31), vs = __shfl_sync(0xffffffffu, my_v, i & 31);
-          if (lane == 0) {
-            scales[stage][warp][0] = ks;
-            scales[stage][warp][1] = vs;
-          }
+          if (lane == 0) scales[to_stage][warp] = make_float2(ks, vs);
         }
-        // rows that no query sees are filled with zeros: whatever lies there must not count
-        const int lo = p < 0 ? kGroup : range.lo - key0, hi = p < 0 ? 0 : range.hi - key0;
-        const size_t at = ((size_t)max(p, 0) * a.kv.page_stride + ((size_t)head * page + key0 % page) * HD) * L::ES;
-        const char *k = reinterpret_cast<const char*>(a.kv.k) + at, *v = reinterpret_cast<const char*>(a.kv.v) + at;
-        const uint32_t to = ring_at + stage * L::STAGE + warp * 2 * L::GB;
+        const uint32_t to = ring_at + to_stage * L::STAGE + warp * 2 * L::GB;
+        const char *k = reinterpret_cast<const char*>(a.kv.k) + (size_t)at * 16, *v = reinterpret_cast<const char*>(a.kv.v) + (size_t)at * 16;
+        if (key0 >= range.lo && key0 + kGroup <= range.hi && at != 0xffffffffu) {
 #pragma unroll
-        for (int c0 = 0; c0 < L::GB / 16; c0 += 32) {
-          const int c = c0 + lane;
-          if ((L::GB / 16) % 32 == 0 || c < L::GB / 16) {
+          for (int c0 = 0; c0 < L::GB / 16; c0 += 32) {
+            const int c = c0 + lane;
+            if ((L::GB / 16) % 32 == 0 || c < L::GB / 16) {
+              const int row = c / L::CPR, in_row = c % L::CPR;
+              copy_16(to + piece<L::CPR, false>(row, in_row) * 16, k + c * 16, true);
+              copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, v + c * 16, true);
+            }
+          }
+        } else {
+          // rows that no query sees are filled with zeros: whatever lies there must not count
+          const int lo = range.lo - key0, hi = at == 0xffffffffu ? 0 : range.hi - key0;
+#pragma unroll 1
+          for (int c = lane; c < L::GB / 16; c += 32) {
             const int row = c / L::CPR, in_row = c % L::CPR;
             const bool take = row >= lo && row < hi;
-            copy_16(to + piece<L::CPR, false>(row, in_row) * 16, k + (take ? c * 16 : 0), take);
-            copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, v + (take ? c * 16 : 0), take);
+            copy_16(to + piece<L::CPR, false>(row, in_row) * 16, take ? k + c * 16 : reinterpret_cast<const char*>(a.kv.k), take);
+            copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, take ? v + c * 16 : reinterpret_cast<const char*>(a.kv.v), take);
           }
         }
+        if (++to_stage == kStages) to_stage = 0;
       }
       copy_commit();
     };
-#pragma unroll
-    for (int i = 0; i < L::STAGES - 1; ++i) copy(i);
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) copy(i);
 
-    Rows<HD, F8> r;
-    const int my_rows0 = rows0 + (kM == 1 ? 0 : warp * 16);
-    load_queries<HD, F8>(a, s, my_rows0, head, r);
+    Rows<HD, F8, NB> r;
+    const int my_rows0 = rows0 + (kSplit ? 0 : warp * 8 * NB);
+    load_queries<HD, F8, NB>(a, s, my_rows0, head, r);
     // positions of the warp's first and last row
     const bool any_row = my_rows0 < s.n * a.group;
-    const int p_first = s.pos + my_rows0 / a.group, p_last = s.pos + min(s.n - 1, (my_rows0 + 15) / a.group);
+    const int p_first = s.pos + my_rows0 / a.group, p_last = s.pos + min(s.n - 1, (my_rows0 + 8 * NB - 1) / a.group);
 
-    for (int i = 0; i < count; ++i) {
-      copy_wait<L::STAGES - 2>();
-      if (kM == 1) __syncwarp();
-      else __syncthreads();
-      copy(i + L::STAGES - 1);
-      const int stage = i % L::STAGES;
-      const char* at = ring + stage * L::STAGE;
 #pragma unroll 1
-      for (int w = kM == 1 ? warp : 0; w < (kM == 1 ? warp + 1 : kWarps); ++w) {
+    for (int i = 0; i < count; ++i) {
+      copy_wait<kStages - 2>();
+      if (kSplit) __syncwarp();
+      else __syncthreads();
+      copy(i + kStages - 1);
+      const char* at = ring + from_stage * L::STAGE;
+#pragma unroll 1
+      for (int w = kSplit ? warp : 0; w < (kSplit ? warp + 1 : kWarps); ++w) {
         const int key0 = (tile0 + i) * kTile + w * kGroup;
         if (!any_row || key0 > p_last || (a.window && key0 + kGroup - 1 <= p_first - a.window)) continue;
         const bool checked = key0 + kGroup - 1 > p_first || (a.window && key0 <= p_last - a.window);
-        keys_16<HD, F8>(at + w * 2 * L::GB, at + w * 2 * L::GB + L::GB, key0, checked, a.window,
-                        F8 ? scales[stage][w][0] : 1.f, F8 ? scales[stage][w][1] : 1.f, r);
+        const float2 scale = F8 ? scales[from_stage][w] : make_float2(1.f, 1.f);
+        keys_16<HD, F8, NB>(at + w * 2 * L::GB, at + w * 2 * L::GB + L::GB, key0, checked, a.window, scale.x, scale.y, r);
       }
+      if (++from_stage == kStages) from_stage = 0;
     }
     copy_wait<0>();
 
@@ -571,27 +607,32 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
     float unit_o = 1.f;
     if (F8) unit_o = r.v_ref * (1.f / kPScale);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 1);
-      r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 2);
-    }
-    if (kM == 1) {
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        r.l[n][h] += __shfl_xor_sync(0xffffffffu, r.l[n][h], 4);
+        r.l[n][h] += __shfl_xor_sync(0xffffffffu, r.l[n][h], 8);
+        r.l[n][h] += __shfl_xor_sync(0xffffffffu, r.l[n][h], 16);
+      }
+    if (kSplit) {
       __syncthreads();  // all warps are done with the ring, which now takes their outputs
       float* o_at = reinterpret_cast<float*>(ring);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = g + 8 * h;
-        if (j == 0) {
-          join_m[warp][row] = r.m[h];
-          join_l[warp][row] = r.l[h];
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 8 * n + 2 * j + h;
+          if (g == 0) {
+            join_m[warp][row] = r.m[n][h];
+            join_l[warp][row] = r.l[n][h];
+          }
+#pragma unroll
+          for (int y = 0; y < HD / 16; ++y)
+            *reinterpret_cast<float2*>(o_at + (warp * kRows + row) * HD + column<HD, F8>(2 * y, g)) =
+                make_float2(r.o[n][y][h] * unit_o, r.o[n][y][2 + h] * unit_o);
         }
-#pragma unroll
-        for (int x = 0; x < HD / 8; ++x)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) o_at[(warp * 16 + row) * HD + column<HD, F8>(x, j, c)] = r.o[x][2 * h + c] * unit_o;
-      }
       __syncthreads();
-      const int n_rows = min(16, s.n * a.group - rows0);
+      const int n_rows = min(kRows, s.n * a.group - rows0);
       for (int i = tid; i < n_rows * (HD / 4); i += kThreads) {
         const int row = i / (HD / 4), col = i % (HD / 4) * 4;
         float top = join_m[0][row];
@@ -602,7 +643,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float by = exp2_fast(join_m[w][row] - base);
-          const float4 v = *reinterpret_cast<const float4*>(o_at + (w * 16 + row) * HD + col);
+          const float4 v = *reinterpret_cast<const float4*>(o_at + (w * kRows + row) * HD + col);
           if (join_m[w][row] == -INFINITY && join_l[w][row] == 0.f) continue;  // saw nothing
           l += join_l[w][row] * by;
           o[0] += v.x * by; o[1] += v.y * by; o[2] += v.z * by; o[3] += v.w * by;
@@ -619,27 +660,24 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const Attn a) {
       }
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = warp * 16 + g + 8 * h, at = rows0 + row;
-        if (at >= s.n * a.group) continue;
-        const float by = complete ? (r.l[h] == 0.f ? 0.f : unit_o / r.l[h]) : unit_o;
-        const int t = at / a.group, hd = at % a.group;
-        bf16* out = a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(head * a.group + hd) * HD;
-        float* part = a.part + ((size_t)slot * kRows + row) * HD;
-        if (!complete && j == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.m[h], r.l[h]);
-        constexpr int EV = L::VV / L::ES;
-        if (EV >= 2) {
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int x = 0; x < HD / 8; x += 2)
+        for (int h = 0; h < 2; ++h) {
+          const int row = warp * 8 * NB + 8 * n + 2 * j + h, at = rows0 + row;
+          if (at >= s.n * a.group) continue;
+          const float by = complete ? (r.l[n][h] == 0.f ? 0.f : unit_o / r.l[n][h]) : unit_o;
+          const int t = at / a.group, hd = at % a.group;
+          bf16* out = a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(head * a.group + hd) * HD;
+          float* part = a.part + ((size_t)slot * kRows + row) * HD;
+          if (!complete && g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.m[n][h], r.l[n][h]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = column<HD, F8>(x, j, c);
-              const float u = r.o[x][2 * h + c] * by, v = r.o[x + 1][2 * h + c] * by;
-              if (complete) *reinterpret_cast<uint32_t*>(out + col) = pack<false>(u, v);
-              else *reinterpret_cast<float2*>(part + col) = make_float2(u, v);
-            }
+          for (int y = 0; y < HD / 16; ++y) {
+            const int col = column<HD, F8>(2 * y, g);
+            const float u = r.o[n][y][h] * by, v = r.o[n][y][2 + h] * by;
+            if (complete) *reinterpret_cast<uint32_t*>(out + col) = pack<false>(u, v);
+            else *reinterpret_cast<float2*>(part + col) = make_float2(u, v);
+          }
         }
-      }
     }
     if (!complete && begins && tid == 0) {
       // parts: this CTA's and one of each of the next ones until the item ends
@@ -717,53 +755,74 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const Attn a) {
 }
 
 // CTAs of a wave: bounded so that the workspace's size is known without asking for the occupancy.
-constexpr int kMostPerSm = 4, kMostPerSmMany = 2;
+constexpr int kMostPerSm = 4;
 
-template <int HD, bool F8, int kM>
+template <int HD, bool F8, int NB, bool kSplit>
 cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
-  using L = Layout<HD, F8>;
-  constexpr int kRows = 16 * kM, most = kM == 1 ? kMostPerSm : kMostPerSmMany;
-  constexpr int join = kM == 1 ? kWarps * 16 * HD * 4 : 0, smem = L::STAGES * L::STAGE > join ? L::STAGES * L::STAGE : join;
+  using F = Form<HD, F8, NB, kSplit>;
+  constexpr int kRows = F::kRows, most = F::kCtas;
+  static_assert(most <= kMostPerSm, "the workspace is sized for this many");
   static unsigned long long opted = 0;
-  auto kernel = kv_attention_kernel<HD, F8, kM>;
-  if (!smem_opt_in(kernel, smem, opted)) return cudaGetLastError();
-  static int fit = 0;  // the same on every device of this architecture
-  if (fit == 0 && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, kThreads, smem) != cudaSuccess) return cudaGetLastError();
-  const int per_sm = fit < most ? (fit > 0 ? fit : 1) : most;
+  auto kernel = kv_attention_kernel<HD, F8, NB, kSplit>;
+  if (!smem_opt_in(kernel, F::kSmem, opted)) return cudaGetLastError();
   // no more CTAs than there can be units: items, or pieces of kLeast tiles of them
   const long long capacity = (long long)a.kv.table_pitch * a.kv.page_size;
   const long long longest = a.window ? min(capacity, (long long)a.window + (kRows - 1) / a.group + kTile) : capacity;
   const long long items = (((long long)a.batch.n_tokens * a.group) / kRows + a.batch.n_seq) * a.kv.kv_heads;
   const long long pieces = ((longest + kTile - 1) / kTile + 1 + kLeast - 1) / kLeast;
   const bool may_share = (longest + kTile - 1) / kTile > kLeast;
-  const int ctas = (int)min((long long)sms * per_sm, may_share ? items * pieces : items);
+  const int ctas = (int)min((long long)sms * most, may_share ? items * pieces : items);
   char* at = reinterpret_cast<char*>(workspace);
   a.head = reinterpret_cast<int4*>(at);
   at += sizeof(int4) * (size_t)sms * most;
   a.stats = reinterpret_cast<float2*>(at);
   at += sizeof(float2) * 2 * (size_t)sms * most * kRows;
   a.part = reinterpret_cast<float*>(at);
-  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, s, a);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), F::kSmem, s, a);
   if (e != cudaSuccess || !may_share) return e;
   const int rows = (int)min((long long)kRows, (long long)a.max_new * a.group);
   return launch_pdl(kv_join_kernel<HD, kRows>, dim3((unsigned)ctas, (unsigned)rows), dim3(kThreads), 0, s, a);
 }
 
+// Rows of one KV head at most: which form.
+template <int HD, bool F8>
+cudaError_t run_rows(const Attn& a, int sms, void* workspace, cudaStream_t s) {
+  constexpr int kMany = HD <= 64 ? 4 : 2;
+  const long long rows = (long long)a.max_new * a.group;
+  if (rows <= 8) return run<HD, F8, 1, true>(a, sms, workspace, s);
+  if (rows <= 16) return run<HD, F8, 2, true>(a, sms, workspace, s);
+  return run<HD, F8, kMany, false>(a, sms, workspace, s);
+}
 template <int HD>
 cudaError_t run_hd(const Attn& a, int sms, void* workspace, cudaStream_t s) {
-  const bool many = (long long)a.max_new * a.group > 16;
-  if (a.kv.e4m3) return many ? run<HD, true, 4>(a, sms, workspace, s) : run<HD, true, 1>(a, sms, workspace, s);
-  return many ? run<HD, false, 4>(a, sms, workspace, s) : run<HD, false, 1>(a, sms, workspace, s);
+  return a.kv.e4m3 ? run_rows<HD, true>(a, sms, workspace, s) : run_rows<HD, false>(a, sms, workspace, s);
 }
 
 }  // namespace
 
 bool kv_head_dim_supported(int hd) { return hd == 32 || hd == 48 || hd == 64 || hd == 96 || hd == 128; }
 
-size_t kv_attention_workspace(int sms, int hd) {
-  auto bytes = [&](size_t ctas, size_t rows) { return sizeof(int4) * ctas + 2 * ctas * rows * (sizeof(float2) + sizeof(float) * hd); };
-  const size_t few = bytes((size_t)sms * kMostPerSm, 16), many = bytes((size_t)sms * kMostPerSmMany, 64);
-  return few > many ? few : many;
+template <int HD>
+static size_t workspace_of(int sms) {
+  auto bytes = [&](size_t per_sm, size_t rows) {
+    return sms * per_sm * (sizeof(int4) + 2 * rows * (sizeof(float2) + sizeof(float) * HD));
+  };
+  using A = Form<HD, false, 1, true>;
+  using B = Form<HD, false, 2, true>;
+  using C = Form<HD, false, HD <= 64 ? 4 : 2, false>;
+  size_t most = bytes(A::kCtas, A::kRows);
+  if (bytes(B::kCtas, B::kRows) > most) most = bytes(B::kCtas, B::kRows);
+  if (bytes(C::kCtas, C::kRows) > most) most = bytes(C::kCtas, C::kRows);
+  return most;
+}
+size_t kv_attention_workspace(int sms, int hd) {  // the same for both types of cache
+  switch (hd) {
+    case 32: return workspace_of<32>(sms);
+    case 48: return workspace_of<48>(sms);
+    case 64: return workspace_of<64>(sms);
+    case 96: return workspace_of<96>(sms);
+  }
+  return workspace_of<128>(sms);
 }
 
 cudaError_t kv_attention(const PagedKv& kv, const Batch& batch, int heads, const bf16* q, int ld_q, bf16* out, int ld_out,

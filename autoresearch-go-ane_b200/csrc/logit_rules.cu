@@ -10,7 +10,21 @@ namespace ane {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr uint32_t kCount = 0xffffffu, kSeen = 1u << 24;  // entry of a token: how often in the output, and whether at all
+
+// What a stretch keeps of a token: how often it is in the output, whether it is in the prompt, and 1 + its last bias' place in the row's
+// list.  32 bits where token lists are shorter than 2^15, 64 otherwise.
+template <class W>
+struct Entry;
+template <>
+struct Entry<uint32_t> {
+  static constexpr int kBias = 16;
+  static constexpr uint32_t kSeen = 1u << 15, kCount = kSeen - 1;
+};
+template <>
+struct Entry<unsigned long long> {
+  static constexpr int kBias = 32;
+  static constexpr unsigned long long kSeen = 1ull << 31, kCount = kSeen - 1;
+};
 
 struct Rules {
   ane_logit_rules_args a;
@@ -33,17 +47,19 @@ __device__ __forceinline__ float4 load4(const Rules& r, size_t at, int n) {
   return make_float4(x[0], x[1], x[2], x[3]);
 }
 
-template <bool BF, int kStretch>
+template <bool BF, int kStretch, class W>
 __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const Rules r) {
+  using E = Entry<W>;
   constexpr int kEach = kStretch / (kThreads * 4);  // groups of four logits of a thread
-  extern __shared__ uint32_t shared[];
-  uint32_t* seen = shared;                                                   // [kStretch]
-  uint32_t* bias_at = shared + (r.a.d_tokens ? kStretch : 0);  // [kStretch]: 1 + entry in the row's list
+  __shared__ __align__(16) W seen[kStretch];
   const ane_logit_rules_args& a = r.a;
   pdl_trigger();
-  pdl_wait();
   const int row = blockIdx.y, v0 = blockIdx.x * kStretch, tid = threadIdx.x;
   const int len = min(kStretch, a.vocab - v0);
+  const bool marks = a.d_tokens || a.d_bias_start;
+  if (marks)
+    for (int i = tid; i < kStretch * (int)sizeof(W) / 16; i += kThreads) reinterpret_cast<uint4*>(seen)[i] = make_uint4(0, 0, 0, 0);
+  pdl_wait();
   float4 x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
@@ -59,27 +75,7 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const Rules r) {
       mask = a.d_mask + (size_t)m * a.ld_mask;
     }
   }
-  if (a.d_tokens)
-    for (int i = tid; i < len; i += kThreads) seen[i] = 0;
-  if (a.d_bias_start)
-    for (int i = tid; i < len; i += kThreads) bias_at[i] = 0;
-  __syncthreads();
-  if (a.d_tokens) {
-    int n = a.d_n_tokens[row];
-    if (n < 0 || n > a.ld_tokens) {
-      if (tid == 0) atomicCAS(r.status, DEV_OK, DEV_BAD_INDEX);
-      n = 0;
-    }
-    const int prompt = a.d_n_prompt ? a.d_n_prompt[row] : 0;
-    const int* tokens = a.d_tokens + (size_t)row * a.ld_tokens;
-#pragma unroll 4
-    for (int i = tid; i < n; i += kThreads) {
-      const int t = tokens[i];
-      if (t < v0 || t - v0 >= len) continue;
-      if (i < prompt) atomicOr(seen + (t - v0), kSeen);
-      else atomicAdd(seen + (t - v0), 1u);
-    }
-  }
+  if (marks) __syncthreads();
   int first_bias = 0;
   if (a.d_bias_start) {
     first_bias = a.d_bias_start[row];
@@ -90,37 +86,61 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const Rules r) {
     }
     for (int i = tid; i < n; i += kThreads) {
       const int t = a.d_bias_token[first_bias + i];
-      if (t >= v0 && t - v0 < len) atomicMax(bias_at + (t - v0), (uint32_t)i + 1u);
+      if (t >= v0 && t - v0 < len) atomicMax(seen + (t - v0), (W)(i + 1) << E::kBias);  // nothing else is there yet
+    }
+    __syncthreads();
+  }
+  if (a.d_tokens) {
+    int n = a.d_n_tokens[row];
+    if (n < 0 || n > a.ld_tokens) {
+      if (tid == 0) atomicCAS(r.status, DEV_OK, DEV_BAD_INDEX);
+      n = 0;
+    }
+    const int prompt = a.d_n_prompt ? a.d_n_prompt[row] : 0;
+    const int* tokens = a.d_tokens + (size_t)row * a.ld_tokens;
+    // eight at a time, so that as many are on their way
+    for (int i0 = 0; i0 < n; i0 += 8 * kThreads) {
+      int t[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kThreads + tid;
+        t[k] = i < n ? tokens[i] - v0 : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if ((unsigned)t[k] >= (unsigned)len) continue;
+        if (i0 + k * kThreads + tid < prompt) atomicOr(seen + t[k], E::kSeen);
+        else atomicAdd(seen + t[k], (W)1);
+      }
     }
   }
   const float rep = a.d_repetition ? a.d_repetition[row] : 1.f, freq = a.d_frequency ? a.d_frequency[row] : 0.f;
   const float pres = a.d_presence ? a.d_presence[row] : 0.f;
-  __syncthreads();
+  if (marks) __syncthreads();
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int v = (i * kThreads + tid) * 4;
     if (v >= len) break;
     float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    if (a.d_tokens) {
-      const uint4 c4 = *reinterpret_cast<const uint4*>(seen + v);
-      const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+    if (marks) {
+      W c[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (v + k < len && c[k]) {
-          if (a.d_repetition) y[k] = y[k] > 0.f ? __fdiv_rn(y[k], rep) : __fmul_rn(y[k], rep);
-          const uint32_t n = c[k] & kCount;
-          if (n) {
-            if (a.d_frequency) y[k] = __fsub_rn(y[k], __fmul_rn(freq, (float)n));
-            if (a.d_presence) y[k] = __fsub_rn(y[k], pres);
+      for (int k = 0; k < (int)sizeof(W) / 4; ++k) reinterpret_cast<uint4*>(c)[k] = reinterpret_cast<const uint4*>(seen + v)[k];
+      if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c[k] & (E::kSeen | E::kCount)) {
+            if (a.d_repetition) y[k] = y[k] > 0.f ? __fdiv_rn(y[k], rep) : __fmul_rn(y[k], rep);
+            const uint32_t n = (uint32_t)(c[k] & E::kCount);
+            if (n) {
+              if (a.d_frequency) y[k] = __fsub_rn(y[k], __fmul_rn(freq, (float)n));
+              if (a.d_presence) y[k] = __fsub_rn(y[k], pres);
+            }
           }
+          const uint32_t at = (uint32_t)(c[k] >> E::kBias);
+          if (at) y[k] = __fadd_rn(y[k], a.d_bias[first_bias + at - 1]);
         }
-    }
-    if (a.d_bias_start) {
-      const uint4 c4 = *reinterpret_cast<const uint4*>(bias_at + v);
-      const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (v + k < len && c[k]) y[k] = __fadd_rn(y[k], a.d_bias[first_bias + c[k] - 1]);
+      }
     }
     if (mask) {
       const uint32_t bits = mask[(v0 + v) >> 5] >> ((v0 + v) & 31);
@@ -139,11 +159,8 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const Rules r) {
   }
 }
 
-template <bool BF, int kStretch>
+template <bool BF, int kStretch, class W>
 cudaError_t run(const Rules& r, cudaStream_t s) {
-  static unsigned long long opted = 0;
-  const size_t smem = sizeof(uint32_t) * kStretch * ((r.a.d_tokens ? 1 : 0) + (r.a.d_bias_start ? 1 : 0));
-  if (!smem_opt_in(logit_rules_kernel<BF, kStretch>, 2 * sizeof(uint32_t) * kStretch, opted)) return cudaGetLastError();
   // rows in slices of what a grid's second dimension holds
   for (int row = 0; row < r.a.rows; row += 65535) {
     Rules part = r;
@@ -169,7 +186,7 @@ cudaError_t run(const Rules& r, cudaStream_t s) {
     if (a.d_presence) a.d_presence += row;
     if (a.d_frequency) a.d_frequency += row;
     const dim3 grid((unsigned)((a.vocab + kStretch - 1) / kStretch), (unsigned)a.rows);
-    const cudaError_t e = launch_pdl(logit_rules_kernel<BF, kStretch>, grid, dim3(kThreads), smem, s, part);
+    const cudaError_t e = launch_pdl(logit_rules_kernel<BF, kStretch, W>, grid, dim3(kThreads), 0, s, part);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -183,8 +200,9 @@ cudaError_t logit_rules(const ane_logit_rules_args& a, int* status, cudaStream_t
   const Rules r = {a, status, reinterpret_cast<uintptr_t>(a.d_logits) % (bf ? 8 : 16) == 0 && a.ld_logits % 4 == 0 &&
                                   reinterpret_cast<uintptr_t>(a.d_out) % 16 == 0 && a.ld_out % 4 == 0};
   const bool few = (long long)a.rows * a.vocab <= 1024ll * 1024;
-  if (bf) return few ? run<true, 1024>(r, s) : run<true, 8192>(r, s);
-  return few ? run<false, 1024>(r, s) : run<false, 8192>(r, s);
+  if (a.d_tokens && a.ld_tokens >= 1 << 15) return bf ? run<true, 4096, unsigned long long>(r, s) : run<false, 4096, unsigned long long>(r, s);
+  if (bf) return few ? run<true, 1024, uint32_t>(r, s) : run<true, 4096, uint32_t>(r, s);
+  return few ? run<false, 1024, uint32_t>(r, s) : run<false, 4096, uint32_t>(r, s);
 }
 
 }  // namespace ane

@@ -299,6 +299,9 @@ static const char* cache_fault(const ane_kv_cache* c, int32_t n_heads) {
   if (!aligned16(c->d_k) || !aligned16(c->d_v)) return "keys and values must be 16-byte aligned";
   if (c->page_stride && (c->page_stride < (int64_t)c->n_kv_heads * c->page_size * c->head_dim || c->page_stride % (e4m3 ? 16 : 8)))
     return "bad page_stride";
+  // kernels count 16-byte pieces in 32 bits
+  const unsigned __int128 page = c->page_stride ? c->page_stride : (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
+  if (page * (unsigned)c->n_pages * (e4m3 ? 1 : 2) >= (unsigned __int128)0xffffffffu * 16) return "more than 64 GiB of keys";
   return nullptr;
 }
 

@@ -139,7 +139,7 @@ int32_t ane_op_gemm(const ane_gemm_args* args);
 typedef struct ane_kv_cache {
   uint32_t struct_size;
   int32_t dtype;             /* ANE_KV_BF16 or ANE_KV_E4M3 */
-  void* d_k;                 /* [n_pages][n_kv_heads][page_size][head_dim] */
+  void* d_k;                 /* [n_pages][n_kv_heads][page_size][head_dim], less than 64 GiB */
   void* d_v;                 /* the same; 16-byte aligned both */
   float* d_k_scale;          /* ANE_KV_E4M3: [n_pages][n_kv_heads]; else unused */
   float* d_v_scale;

@@ -51,7 +51,7 @@ CACHES = [
     (dict(n_kv_heads=3), "n_heads"), (dict(table_pitch=0), "dimensions"), (dict(d_k=None), "null"), (dict(d_v=None), "null"),
     (dict(d_k_scale=None), "null"), (dict(d_v_scale=None), "null"), (dict(d_page_table=None), "null"), (dict(d_k=HERE + 8), "aligned"),
     (dict(d_v=HERE + 1), "aligned"), (dict(page_stride=2047), "page_stride"), (dict(page_stride=2056), "page_stride"),
-    (dict(page_stride=-2048), "page_stride"),
+    (dict(page_stride=-2048), "page_stride"), (dict(page_stride=1 << 40), "64 GiB"), (dict(page_stride=1 << 62, n_pages=2 ** 31 - 1), "64 GiB"),
 ]
 
 
