@@ -4,16 +4,16 @@
 // head r % group.  Products are m16n8k16 on mma.sync: single tokens are bound by the bytes of the cache, and their
 // products take a fraction of the time that the operands need to arrive.
 //
-//   few rows (up to 16 a KV head): a CTA holds 8 or 16 rows; its four warps take 16 of every 64 keys each, with softmax statistics
-//     of their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
+//   few rows (up to 16 a KV head): a CTA holds 8 or 16 rows; its eight warps take 16 of every 128 keys each, with softmax
+//     statistics of their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
 //   many rows: a CTA holds 64 or 128 rows, a warp a quarter of them, and all warps go over all keys.
 //
 // Keys and values come by cp.async into a ring of stages of 64 keys.  8-bit ones stay 8-bit until they are in registers, where they
 // become f16, which holds e4m3 exactly: queries are brought to f16 by a power of two per row, scales of keys go onto the
 // scores, scales of values onto the probabilities.
 //
-// Work is cut on the device, as only the device knows the lengths: all tiles of 64 keys of all (sequence, row tile, KV head) in
-// one line, an even share of the line to each CTA of one wave.  What a CTA did of an item that others share goes to the
+// Work is cut on the device, as only the device knows the lengths: all tiles of keys of all (sequence, row tile, KV head) in one
+// line, an even share of the line to each CTA of one wave.  What a CTA did of an item that others share goes to the
 // workspace, and a second kernel joins the parts in their order, without atomics: the same sums from call to call.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -23,17 +23,31 @@
 namespace ane {
 namespace {
 
-constexpr int kTile = 64, kGroup = 16, kWarps = 4, kThreads = kWarps * 32;
-constexpr int kLeast = 4;  // tiles of an item that are not worth sharing: joining parts takes the time of about four
-constexpr float kPScale = 32768.f;  // of f16 probabilities: those down to 2^-29 of the row's largest stay normal
+constexpr int kGroup = 16;  // keys of a product
+// A row's maximum follows its scores only where they exceed it by more than this (in log2), so that probabilities are below 2^kSlack: most
+// keys then need no exchange of maxima and no new factor on what has been summed.
+constexpr float kSlack = 8.f;
+constexpr float kPScale = 128.f;  // of f16 probabilities, 2^15 at most then: those down to 2^-21 of the maximum's stay normal
 constexpr float kLowest = 1.17549435e-38f;
+
+// Quotients by a number known at launch, in five instructions: floor(2^32 / d) gives them or one less.
+struct Div {
+  uint32_t d, m;
+  Div() = default;
+  explicit Div(int by) : d(by), m(by == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / by)) {}
+  __device__ __forceinline__ int operator()(int n) const {
+    const uint32_t q = __umulhi((uint32_t)n, m);
+    return (int)(q + ((uint32_t)n - q * d >= d ? 1u : 0u));
+  }
+};
 
 struct Attn {
   PagedKv kv;
   Batch batch;
   const bf16* q;
   bf16* out;
-  int ld_q, ld_out, group, max_new, window;
+  int ld_q, ld_out, group, max_new, window, capacity, stages;
+  Div by_group, by_page;
   float scale_log2;
   int4* head;      // [CTAs]: the shared item that begins in this CTA: sequence (< 0: none), row tile, KV head, parts
   float2* stats;   // [2 * CTAs][rows]: maximum (log2) and sum of a part
@@ -47,7 +61,32 @@ struct Layout {
   static constexpr int RB = HD * ES, GB = kGroup * RB, CPR = RB / 16;  // bytes of a row, of 16 rows; 16-byte pieces of a row
   static constexpr int VK = RB % 64 == 0 ? 16 : RB % 32 == 0 ? 8 : 4;   // bytes that a thread loads of K rows at a time
   static constexpr int VV = RB % 128 == 0 ? 16 : RB % 64 == 0 ? 8 : RB % 32 == 0 ? 4 : 2;  // of V rows
-  static constexpr int STAGE = kWarps * 2 * GB;
+};
+
+// kSplit: eight warps share 8 * NB rows and take an eighth of the keys each; otherwise each of four has 8 * NB rows and takes all keys of a tile.
+// kGroups: times 16 keys that a warp takes at once.  More keys share their softmax's maximum, exchanges and loop, fewer leave the ring room
+// for more stages.
+template <int HD_, bool F8_, int NB_, bool kSplit_>
+struct Form {
+  static constexpr int HD = HD_, NB = NB_, kWarps = kSplit_ ? 8 : 4;
+  static constexpr bool F8 = F8_, kSplit = kSplit_;
+  using L = Layout<HD, F8>;
+  static constexpr int kGroups = kSplit ? (L::RB <= 64 && NB == 1 ? 2 : 1) : 2;
+  // groups of 16 keys of a tile that a warp fetches; the ring has to hold the outputs of kSplit's warps
+  static constexpr int kLoads = kSplit ? kGroups : 1;
+  static constexpr int kThreads = 32 * kWarps, kTile = kGroup * kWarps * kLoads;
+  static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
+  static constexpr int kStage = kWarps * kLoads * 2 * L::GB;
+  // resident CTAs wanted: registers for outputs and queries decide
+  static constexpr int kRegs = NB * (HD / 16 * 6 + 16);
+  static constexpr int kCtas = kSplit && (kRegs > 80 || 3 * kStage > 108 * 1024) ? 1 : 2;
+  static constexpr int kRoom = 224 * 1024 / kCtas - 3072, kFit = kRoom / kStage;
+  static constexpr int kStages = kFit < 3 ? 3 : kFit > 6 ? 6 : kFit;
+  static constexpr int kMost = 216 * 1024 / kStage, kDeep = kMost > 8 ? 8 : kMost < kStages ? kStages : kMost;  // where a CTA has an SM to itself
+  static_assert(!kSplit || kWarps * kRows * HD * 4 <= 3 * kStage, "the warps' outputs are joined in the ring");
+  // Tiles of an item that are not worth sharing (joining parts takes a second kernel), and the least share of one that is shared.
+  static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile;
+  static constexpr int kRestart = kSplit ? 768 / kTile : 1;  // what another item costs a CTA, in tiles
 };
 
 // Where 16-byte piece c of a row lies within 16 rows, so that the threads of a fragment load find it in different banks: a thread
@@ -71,10 +110,8 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t pair) {  // the low two bytes
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)pair));
-  return r;
+__device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {  // the low and the high two bytes
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 template <bool F8>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -115,114 +152,179 @@ __device__ __forceinline__ void lds(const char* p, uint32_t* w) {  // B bytes
 // An item is a (sequence, tile of kRows rows, KV head); its key tiles are those that one of its rows sees.
 struct Range {
   int lo, hi;  // positions that some row of the tile sees
-  __device__ int t0() const { return lo / kTile; }
-  __device__ int tiles() const { return (hi - 1) / kTile - lo / kTile + 1; }
+  template <class F>
+  __device__ int t0() const { return lo / F::kTile; }
+  template <class F>
+  __device__ int tiles() const { return (hi - 1) / F::kTile - lo / F::kTile + 1; }
 };
-__device__ __forceinline__ Range range_of(const Span& s, int rows0, int rows, int group, int window) {
-  const int t_first = rows0 / group, t_last = min(s.n - 1, (rows0 + rows - 1) / group);
-  return {window ? max(0, s.pos + t_first + 1 - window) : 0, s.pos + t_last + 1};
+// The positions that a tile of rows sees; with one tile for all rows of a sequence (kSplit) this takes no quotients.
+template <class F>
+__device__ __forceinline__ Range range_of(const Attn& a, const Span& s, int mt) {
+  if (F::kSplit) return {a.window ? max(0, s.pos + 1 - a.window) : 0, s.pos + s.n};
+  const int t_last = min(s.n - 1, a.by_group((mt + 1) * F::kRows - 1));
+  return {a.window ? max(0, s.pos + a.by_group(mt * F::kRows) + 1 - a.window) : 0, s.pos + t_last + 1};
+}
+template <class F>
+__device__ __forceinline__ int row_tiles(const Attn& a, const Span& s) {
+  return F::kSplit ? (s.n > 0 ? 1 : 0) : (s.n * a.group + F::kRows - 1) / F::kRows;
 }
 
+// An item, and the tiles of it that are this CTA's.
+struct Item {
+  int b, mt, head, off;  // off: the first of its tiles that is
+  Span s;
+  Range range;
+  int tiles, count;  // all tiles, this CTA's
+  int unit;          // of its first tile here, in the line
+};
+
+// How the line of all tiles is cut.  Whole items to a CTA where all are short; one piece of at most `share` tiles of one item to each CTA where
+// that makes the largest share little larger than an even one, since another item costs a CTA a new start; else even shares.
+enum Cut { kWhole, kPieces, kEven };
+// The host has made sure that there are less than 2^31 units.
 struct Plan {
-  long long units, first, last;  // of the line: all, and this CTA's
-  long long share;
-  bool whole;                    // units are items, not tiles
-  int b, mt, head, off;          // where `first` lies
+  int first, last;  // this CTA's units of the line: items, pieces or tiles
+  int share;        // tiles (kWhole: items) of a CTA
+  int cut;
 };
 
-template <int kRows>
-__device__ __forceinline__ void weigh(const Attn& a, const Span& s, int& items, long long& tiles, int& longest) {
-  items = 0;
-  tiles = 0;
-  for (int r = 0; r < s.n * a.group; r += kRows) {
-    const int t = range_of(s, r, kRows, a.group, a.window).tiles();
-    ++items;
-    tiles += t;
-    longest = max(longest, t);
+template <class F>
+__device__ __forceinline__ void measure(const Attn& a, const Plan& p, Item& it) {
+  it.range = range_of<F>(a, it.s, it.mt);
+  it.tiles = it.range.template tiles<F>();
+  it.count = p.cut == kWhole ? it.tiles : p.cut == kPieces ? min(it.tiles - it.off, p.share) : min(it.tiles - it.off, p.last - it.unit);
+}
+template <class F>
+__device__ __forceinline__ bool next_item(const Attn& a, const Plan& p, Item& it) {
+  it.unit += p.cut == kEven ? it.count : 1;
+  if (it.unit >= p.last) return false;
+  it.off = 0;
+  if (++it.head == a.kv.kv_heads) {
+    it.head = 0;
+    ++it.mt;
+    while (it.mt >= row_tiles<F>(a, it.s)) {
+      it.mt = 0;
+      it.s = span_of(a.batch, ++it.b, a.capacity, a.max_new, a.status);
+    }
   }
+  measure<F>(a, p, it);
+  return true;
 }
 
-template <int kRows>
-__device__ Plan make_plan(const Attn& a, int capacity) {
-  __shared__ long long sums[2][kWarps];
-  __shared__ int longest_of[kWarps];
-  __shared__ Plan plan;
+// n / d rounded up for n + d < 2^31, d > 0: a quotient of floats, put right by one step at most (its error is below 2^-22 of it, so
+// from 2^21 on an exact one).
+__device__ __forceinline__ int quotient_up(int n, int d) {
+  if (n >= 1 << 21) return (int)((uint32_t)(n + d - 1) / (uint32_t)d);
+  int q = (int)__fdividef((float)n, (float)d);
+  if (q * d < n) ++q;
+  if (q * d < n) ++q;
+  if ((q - 1) * d >= n && q > 0) --q;
+  return q;
+}
+
+template <class F>
+__device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
+  constexpr int kWarps = F::kWarps, kThreads = F::kThreads;
+  __shared__ int3 all[kWarps];
+  __shared__ int sums[kWarps];
+  __shared__ int4 at, span;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.batch.n_seq + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, a.batch.n_seq), b1 = min(b0 + per, a.batch.n_seq);
-  long long items = 0, tiles = 0;
-  int longest = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Span s = span_of(a.batch, b, capacity, a.max_new, a.status);
-    int i;
-    long long t;
-    weigh<kRows>(a, s, i, t, longest);
-    items += (long long)i * a.kv.kv_heads;
-    tiles += t * a.kv.kv_heads;
-  }
-  long long before_items = items, before_tiles = tiles;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long i = __shfl_up_sync(0xffffffffu, before_items, o), t = __shfl_up_sync(0xffffffffu, before_tiles, o);
-    if (lane >= o) {
-      before_items += i;
-      before_tiles += t;
+  Span s = {0, 0, 0};  // of the thread's only sequence, mostly
+  // what(tiles of an item) of all items of a KV head of the thread's sequences, until it says stop
+  auto each = [&](auto what) {
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      if (per > 1) s = span_of(a.batch, b, a.capacity, a.max_new, a.status);
+      const int mts = row_tiles<F>(a, s);
+#pragma unroll 1
+      for (int mt = 0; mt < mts; ++mt)
+        if (what(b, mt, range_of<F>(a, s, mt).template tiles<F>())) return;
     }
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  if (lane == 31) {
-    sums[0][warp] = before_items;
-    sums[1][warp] = before_tiles;
-    longest_of[warp] = longest;
-  }
-  if (tid == 0) plan.b = -1;
+  };
+  if (per == 1 && b0 < b1) s = span_of(a.batch, b0, a.capacity, a.max_new, a.status);
+  int items = 0, tiles = 0, longest = 0;
+  each([&](int, int, int t) {
+    ++items;
+    tiles += t;
+    longest = max(longest, t);
+    return false;
+  });
+  items = __reduce_add_sync(0xffffffffu, items);
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) all[warp] = make_int3(items, tiles, longest);
+  if (tid == 0) at = make_int4(-1, 0, 0, 0);
   __syncthreads();
-  long long all_items = 0, all_tiles = 0;
+  items = tiles = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      before_items += sums[0][w];
-      before_tiles += sums[1][w];
-    }
-    all_items += sums[0][w];
-    all_tiles += sums[1][w];
-    longest = max(longest, longest_of[w]);
+    items += all[w].x;
+    tiles += all[w].y;
+    longest = max(longest, all[w].z);
   }
-  const bool whole = longest <= kLeast;
-  const long long units = whole ? all_items : all_tiles;
-  long long share = (units + gridDim.x - 1) / gridDim.x;
-  if (!whole) share = max(share, (long long)kLeast);
-  const long long first = share * blockIdx.x;
-  const long long mine = whole ? items : tiles, before = (whole ? before_items : before_tiles) - mine;
-  if (first < units && first >= before && first < before + mine) {
-    long long rest = first - before;
-    for (int b = b0; b < b1; ++b) {
-      const Span s = span_of(a.batch, b, capacity, a.max_new, a.status);
-      int mt = 0;
-      bool found = false;
-      for (int r = 0; r < s.n * a.group; r += kRows, ++mt) {
-        const int t = whole ? 1 : range_of(s, r, kRows, a.group, a.window).tiles();
-        const long long w = (long long)t * a.kv.kv_heads;
-        if (rest < w) {
-          plan.b = b;
-          plan.mt = mt;
-          plan.head = (int)(rest / t);
-          plan.off = (int)(rest % t);
-          found = true;
-          break;
-        }
-        rest -= w;
+  items *= a.kv.kv_heads;
+  tiles *= a.kv.kv_heads;
+  const int ctas = gridDim.x;
+  Plan p;
+  p.cut = kWhole;
+  p.share = quotient_up(items, ctas);
+  if (longest > F::kAlone) {
+    const int even = max(quotient_up(tiles, ctas), F::kLeast);
+    // at most tiles / share + items pieces
+    const int pieces = items < ctas ? max(quotient_up(tiles, ctas - items), even) : INT32_MAX;
+    p.cut = pieces <= even + F::kRestart ? kPieces : kEven;
+    p.share = p.cut == kPieces ? pieces : even;
+  }
+  auto weight = [&](int t) { return p.cut == kWhole ? 1 : p.cut == kPieces ? quotient_up(t, p.share) : t; };
+  int mine = 0;
+  each([&](int, int, int t) {
+    mine += weight(t);
+    return false;
+  });
+  mine *= a.kv.kv_heads;
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += t;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  int units = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    units += sums[w];
+  }
+  before -= mine;
+  const int step = p.cut == kPieces ? 1 : p.share;
+  p.first = (int)min((long long)step * blockIdx.x, (long long)units);
+  p.last = min(step, units - p.first) + p.first;
+  if (p.first < p.last && p.first >= before && p.first - before < mine) {
+    int rest = p.first - before;
+    each([&](int b, int mt, int t) {
+      const int one = weight(t);
+      if (rest >= one * a.kv.kv_heads) {
+        rest -= one * a.kv.kv_heads;
+        return false;
       }
-      if (found) break;
-    }
+      const int head = (int)((uint32_t)rest / (uint32_t)one), unit = rest - head * one;
+      at = make_int4(b, mt, head, p.cut == kPieces ? unit * p.share : p.cut == kEven ? unit : 0);
+      span = make_int4(s.row, s.n, s.pos, 0);
+      return true;
+    });
   }
   __syncthreads();
-  Plan p = plan;
-  p.units = units;
-  p.share = share;
-  p.whole = whole;
-  p.first = first;
-  p.last = min(first + share, units);
+  const int4 from = at, of = span;
+  it.b = from.x;
+  it.mt = from.y;
+  it.head = from.z;
+  it.off = from.w;
+  it.s = {of.x, of.y, of.z};
+  it.unit = p.first;
+  if (it.b >= 0) measure<F>(a, p, it);
   return p;
 }
 
@@ -233,32 +335,49 @@ template <int HD, bool F8, int NB>
 struct Rows {  // 8 * NB rows of queries
   uint32_t q[NB][HD / 16][2];  // right operands: the thread's row g of each eight
   float o[NB][HD / 16][4];     // columns of the output column(2 y, g) and column(2 y + 1, g), for rows 2 j and 2 j + 1
-  float m[NB][2], l[NB][2], mult[NB][2];  // rows 2 j and 2 j + 1; mult: what brings products to scores in log2
+  // rows 2 j and 2 j + 1: exponents' base, which is the maximum at the time, the score from which on it is renewed (-infinity: none yet), the sum,
+  // and what brings products to scores in log2
+  float base[NB][2], limit[NB][2], l[NB][2], mult[NB][2];
   int pos[NB][2];                         // their positions; -1: no such row
   float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = kPScale / v_ref
 };
 
+template <int HD, int NB>
+struct RawRows {
+  uint2 w[NB][HD / 16];  // the thread's row g of each eight
+};
 template <int HD, bool F8, int NB>
-__device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int rows0, int head, Rows<HD, F8, NB>& r) {
+__device__ __forceinline__ void fetch_queries(const Attn& a, const Item& it, int rows0, RawRows<HD, NB>& raw) {
   using L = Layout<HD, F8>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, n_rows = s.n * a.group;
+  const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, n_rows = it.s.n * a.group;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int row = rows0 + 8 * n + g;
     const bool there = row < n_rows;
-    const int t = there ? row / a.group : 0, hd = there ? row - t * a.group : 0;
-    const bf16* q = a.q + (size_t)(s.row + t) * a.ld_q + (size_t)(head * a.group + hd) * HD;
+    const int t = there ? a.by_group(row) : 0, hd = there ? row - t * a.group : 0;
+    const bf16* q = a.q + (size_t)(it.s.row + t) * a.ld_q + (size_t)(it.head * a.group + hd) * HD;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      // the four elements that word i (8 bits), or words 2 i and 2 i + 1, of the thread's bytes of a K row meet
+      const int word = F8 ? i : 2 * i, at = (L::VK * j + word / (L::VK / 4) * 4 * L::VK + word % (L::VK / 4) * 4) / L::ES;
+      raw.w[n][i] = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
+    }
+  }
+}
+
+template <int HD, bool F8, int NB>
+__device__ __forceinline__ void begin_rows(const Attn& a, const Item& it, int rows0, const RawRows<HD, NB>& raw, Rows<HD, F8, NB>& r) {
+  const int lane = threadIdx.x & 31, j = lane & 3, n_rows = it.s.n * a.group;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
     float mult = a.scale_log2;
     if (F8) {
-      uint2 w[HD / 16];
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        // word i of the thread's bytes of a K row: four elements
-        const int at = L::VK * j + i / (L::VK / 4) * 4 * L::VK + i % (L::VK / 4) * 4;
-        w[i] = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(w[i].x << 16)), fabsf(__uint_as_float(w[i].x & 0xffff0000u))),
-                               fmaxf(fabsf(__uint_as_float(w[i].y << 16)), fabsf(__uint_as_float(w[i].y & 0xffff0000u)))));
+        const uint2 w = raw.w[n][i];
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(__uint_as_float(w.x << 16)), fabsf(__uint_as_float(w.x & 0xffff0000u))),
+                               fmaxf(fabsf(__uint_as_float(w.y << 16)), fabsf(__uint_as_float(w.y & 0xffff0000u)))));
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -269,24 +388,23 @@ __device__ __forceinline__ void load_queries(const Attn& a, const Span& s, int r
       mult /= by;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        r.q[n][i][0] = pack<true>(__uint_as_float(w[i].x << 16) * by, __uint_as_float(w[i].x & 0xffff0000u) * by);
-        r.q[n][i][1] = pack<true>(__uint_as_float(w[i].y << 16) * by, __uint_as_float(w[i].y & 0xffff0000u) * by);
+        const uint2 w = raw.w[n][i];
+        r.q[n][i][0] = pack<true>(__uint_as_float(w.x << 16) * by, __uint_as_float(w.x & 0xffff0000u) * by);
+        r.q[n][i][1] = pack<true>(__uint_as_float(w.y << 16) * by, __uint_as_float(w.y & 0xffff0000u) * by);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        // words 2 i and 2 i + 1 of the thread's bytes of a K row
-        const int word = 2 * i, at = (L::VK * j + word / (L::VK / 4) * 4 * L::VK + word % (L::VK / 4) * 4) / 2;
-        const uint2 w = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
-        r.q[n][i][0] = w.x;
-        r.q[n][i][1] = w.y;
+        r.q[n][i][0] = raw.w[n][i].x;
+        r.q[n][i][1] = raw.w[n][i].y;
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int mine = rows0 + 8 * n + 2 * j + h;
-      r.pos[n][h] = mine < n_rows ? s.pos + mine / a.group : -1;
-      r.m[n][h] = -INFINITY;
+      r.pos[n][h] = mine < n_rows ? it.s.pos + a.by_group(mine) : -1;
+      r.base[n][h] = 0.f;
+      r.limit[n][h] = -INFINITY;
       r.l[n][h] = 0.f;
       r.mult[n][h] = F8 ? __shfl_sync(0xffffffffu, mult, (2 * j + h) * 4) : mult;
     }
@@ -317,49 +435,72 @@ __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 mat
   return r;
 }
 
-// 16 keys at positions key0.. against the warp's rows.  `checked`: some row does not see some key.
-template <int HD, bool F8, int NB>
-__device__ __forceinline__ void keys_16(const char* ks, const char* vs, int key0, bool checked, int window, float k_scale,
-                                        float v_scale, Rows<HD, F8, NB>& r) {
+// KG * 16 keys at positions key0.. against the warp's rows; group i of them lies at ring + i * 2 * GB.  `checked`: some row does not
+// see some key.
+template <int HD, bool F8, int NB, int KG>
+__device__ __forceinline__ void take_keys(const char* ring, const float2* scales, int key0, bool checked, int window, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
+  constexpr int kChains = NB == 1 ? 2 : 1;
   const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  float s[NB][4];  // keys g (0, 1) and g + 8 (2, 3), rows 2 j and 2 j + 1
+  float s[KG][NB][4];  // keys g (0, 1) and g + 8 (2, 3), rows 2 j and 2 j + 1
+  float2 scale[KG];    // of keys, of values
 #pragma unroll
-  for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-  for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
-    const int byte = L::VK * j + 4 * L::VK * i;
-    uint32_t u[L::VK / 4], w[L::VK / 4];  // of keys g and g + 8
-    lds<L::VK>(ks + piece<L::CPR, false>(g, byte >> 4) * 16 + (byte & 15), u);
-    lds<L::VK>(ks + piece<L::CPR, false>(8 + g, byte >> 4) * 16 + (byte & 15), w);
-#pragma unroll
-    for (int x = 0; x < L::VK / 4; x += F8 ? 1 : 2) {
-      const uint32_t k[4] = {F8 ? e4m3_to_f16(u[x]) : u[x], F8 ? e4m3_to_f16(w[x]) : w[x], F8 ? e4m3_to_f16(u[x] >> 16) : u[x + !F8],
-                             F8 ? e4m3_to_f16(w[x] >> 16) : w[x + !F8]};
-      const int step = F8 ? i * (L::VK / 4) + x : (i * (L::VK / 4) + x) / 2;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) mma<F8>(s[n], k, r.q[n][step][0], r.q[n][step][1]);
-    }
-  }
-  uint32_t seen = 0xffffffffu;  // bit 4 n + i of s[n][i]
-  if (checked) {
+  for (int k = 0; k < KG; ++k) {
+    const char* ks = ring + k * 2 * L::GB;
+    scale[k] = F8 ? scales[k] : make_float2(1.f, 1.f);
+    float even[NB][4];  // a second chain of products, half as long each
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = key0 + g + 8 * (i >> 1), pos = r.pos[n][i & 1];
-        if (key > pos || (window && key <= pos - window)) {
-          s[n][i] = -INFINITY;
-          seen &= ~(1u << (4 * n + i));
+      for (int i = 0; i < 4; ++i) s[k][n][i] = even[n][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
+      const int byte = L::VK * j + 4 * L::VK * i;
+      uint32_t u[L::VK / 4], w[L::VK / 4];  // of keys g and g + 8
+      lds<L::VK>(ks + piece<L::CPR, false>(g, byte >> 4) * 16 + (byte & 15), u);
+      lds<L::VK>(ks + piece<L::CPR, false>(8 + g, byte >> 4) * 16 + (byte & 15), w);
+#pragma unroll
+      for (int x = 0; x < L::VK / 4; x += F8 ? 1 : 2) {
+        uint32_t a[4] = {u[x], w[x], u[x + !F8], w[x + !F8]};
+        if (F8) {
+          e4m3_to_f16(u[x], a[0], a[2]);
+          e4m3_to_f16(w[x], a[1], a[3]);
+        }
+        const int step = F8 ? i * (L::VK / 4) + x : (i * (L::VK / 4) + x) / 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if (kChains == 2 && step % 2 == 0) mma<F8>(even[n], a, r.q[n][step][0], r.q[n][step][1]);
+          else mma<F8>(s[k][n], a, r.q[n][step][0], r.q[n][step][1]);
         }
       }
+    }
+    if (kChains == 2) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[k][n][i] += even[n][i];
+    }
   }
-  float into = 1.f;
+  if (checked) {
+#pragma unroll
+    for (int k = 0; k < KG; ++k)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + kGroup * k + g + 8 * (i >> 1), pos = r.pos[n][i & 1];
+          if (key > pos || (window && key <= pos - window)) s[k][n][i] = -INFINITY;
+        }
+  }
+  float into[KG];
   if (F8) {
-    if (v_scale > r.v_ref) {  // statistics keep their unit, the output changes to the new one
-      const float by = r.v_ref / v_scale;
-      r.v_ref = v_scale;
-      r.v_inv = kPScale / v_scale;
+    float most = scale[0].y;
+#pragma unroll
+    for (int k = 1; k < KG; ++k) most = fmaxf(most, scale[k].y);
+    if (most > r.v_ref) {  // statistics keep their unit, the output changes to the new one
+      const float by = r.v_ref / most;
+      r.v_ref = most;
+      r.v_inv = kPScale / most;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -367,242 +508,284 @@ __device__ __forceinline__ void keys_16(const char* ks, const char* vs, int key0
 #pragma unroll
           for (int i = 0; i < 4; ++i) r.o[n][y][i] *= by;
     }
-    into = v_scale * r.v_inv;
+#pragma unroll
+    for (int k = 0; k < KG; ++k) into[k] = scale[k].y * r.v_inv;
   }
-  uint32_t p[NB][2];
-  bool moved = false;
-  float fix[NB][2];
+  uint32_t p[KG][NB][2];
+  bool above = false;
+  float mult[KG][NB][2];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        mult[k][n][h] = F8 ? fmaxf(r.mult[n][h] * scale[k].x, kLowest) : r.mult[n][h];  // not 0, so that hidden scores stay -infinity
+        top = fmaxf(top, fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h]);
+      }
+      above |= top > r.limit[n][h];
+    }
+  if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float fix[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KG; ++k) top = fmaxf(top, fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const bool none = r.limit[n][h] == -INFINITY;
+        const float base = none ? (top == -INFINITY ? 0.f : top) : fmaxf(top, r.base[n][h]);
+        fix[h] = none ? 1.f : exp2_fast(r.base[n][h] - base);  // sums are still 0 then
+        r.base[n][h] = base;
+        r.limit[n][h] = none && top == -INFINITY ? -INFINITY : base + kSlack;
+        r.l[n][h] *= fix[h];
+      }
+#pragma unroll
+      for (int y = 0; y < HD / 16; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.o[n][y][i] *= fix[i & 1];
+    }
+  }
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float mult = F8 ? fmaxf(r.mult[n][h] * k_scale, kLowest) : r.mult[n][h];  // not 0, so that hidden scores stay -infinity
-      float top = fmaxf(s[n][h], s[n][2 + h]);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      top = fmaxf(top * mult, r.m[n][h]);
-      const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2 of -infinity, which is 0
-      fix[n][h] = exp2_fast(r.m[n][h] - base);
-      moved |= r.m[n][h] != top;
-      r.m[n][h] = top;
-      s[n][h] = exp2_fast(fmaf(s[n][h], mult, -base));
-      s[n][2 + h] = exp2_fast(fmaf(s[n][2 + h], mult, -base));
-      r.l[n][h] = fmaf(r.l[n][h], fix[n][h], s[n][h] + s[n][2 + h]);  // the thread's own keys; joined at the end
-      if (F8) {
-        s[n][h] *= into;
-        s[n][2 + h] *= into;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        s[k][n][h] = exp2_fast(fmaf(s[k][n][h], mult[k][n][h], -r.base[n][h]));
+        s[k][n][2 + h] = exp2_fast(fmaf(s[k][n][2 + h], mult[k][n][h], -r.base[n][h]));
+        sum += s[k][n][h] + s[k][n][2 + h];
       }
+      r.l[n][h] += sum;  // the thread's own keys; joined at the end
     }
     // probabilities in 16 bits: their rounding is half a step of the output's own type or less
-    p[n][0] = transposed(pack<F8>(s[n][0], s[n][1]));
-    p[n][1] = transposed(pack<F8>(s[n][2], s[n][3]));
+#pragma unroll
+    for (int k = 0; k < KG; ++k) {
+      if (F8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[k][n][i] *= into[k];
+      }
+      p[k][n][0] = transposed(pack<F8>(s[k][n][0], s[k][n][1]));
+      p[k][n][1] = transposed(pack<F8>(s[k][n][2], s[k][n][3]));
+    }
   }
-  if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int y = 0; y < HD / 16; ++y)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.o[n][y][i] *= fix[n][i & 1];
-  }
-  bool odd = false;
   if (checked) {
     // a value that is infinite or NaN must not reach rows that do not see its key, and 0 * NaN is NaN
+    bool odd = false;
 #pragma unroll 1
-    for (int i = lane; i < L::GB / 4; i += 32) odd |= not_finite<F8>(*reinterpret_cast<const uint32_t*>(vs + 4 * i));
-    odd = __any_sync(0xffffffffu, odd);
-  }
-  if (odd) {
-    // one product after the other, unseen ones left out
+    for (int k = 0; k < KG; ++k)
 #pragma unroll 1
-    for (int k = 0; k < kGroup; ++k) {
-      const int from = (k & 7) * 4 + j;
-      const uint32_t see = __shfl_sync(0xffffffffu, seen, from) >> (k < 8 ? 0 : 2);
+      for (int i = lane; i < L::GB / 4; i += 32)
+        odd |= not_finite<F8>(*reinterpret_cast<const uint32_t*>(ring + k * 2 * L::GB + L::GB + 4 * i));
+    if (__any_sync(0xffffffffu, odd)) {
+      // one product after the other, unseen ones left out
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const float w0 = __shfl_sync(0xffffffffu, k < 8 ? s[n][0] : s[n][2], from), w1 = __shfl_sync(0xffffffffu, k < 8 ? s[n][1] : s[n][3], from);
+      for (int k = 0; k < KG; ++k) {
+        const char* vs = ring + k * 2 * L::GB + L::GB;
+#pragma unroll 1
+        for (int key = 0; key < kGroup; ++key) {
+          const int from = (key & 7) * 4 + j, at_key = key0 + kGroup * k + key;
 #pragma unroll
-        for (int x = 0; x < HD / 8; ++x) {
-          const int byte = column<HD, F8>(x, g) * L::ES;
-          const char* at = vs + piece<L::CPR, true>(k, byte >> 4) * 16 + (byte & 15);
-          const float v = F8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*reinterpret_cast<const unsigned char*>(at), __NV_E4M3)))
-                             : __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(at) << 16);
-          if (see >> (4 * n) & 1u) r.o[n][x >> 1][2 * (x & 1)] += w0 * v;
-          if (see >> (4 * n + 1) & 1u) r.o[n][x >> 1][2 * (x & 1) + 1] += w1 * v;
+          for (int n = 0; n < NB; ++n) {
+            const float w0 = __shfl_sync(0xffffffffu, key < 8 ? s[k][n][0] : s[k][n][2], from);
+            const float w1 = __shfl_sync(0xffffffffu, key < 8 ? s[k][n][1] : s[k][n][3], from);
+            const bool see0 = at_key <= r.pos[n][0] && !(window && at_key <= r.pos[n][0] - window);
+            const bool see1 = at_key <= r.pos[n][1] && !(window && at_key <= r.pos[n][1] - window);
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x) {
+              const int byte = column<HD, F8>(x, g) * L::ES;
+              const char* at = vs + piece<L::CPR, true>(key, byte >> 4) * 16 + (byte & 15);
+              const float v = F8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*reinterpret_cast<const unsigned char*>(at), __NV_E4M3)))
+                                 : __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(at) << 16);
+              if (see0) r.o[n][x >> 1][2 * (x & 1)] += w0 * v;
+              if (see1) r.o[n][x >> 1][2 * (x & 1) + 1] += w1 * v;
+            }
+          }
         }
       }
+      return;
     }
-    return;
   }
   constexpr int EV = L::VV / L::ES, WV = L::VV >= 4 ? L::VV / 4 : 1;
 #pragma unroll
-  for (int i = 0; i < L::RB / (8 * L::VV); ++i) {
-    const int byte = L::VV * g + 8 * L::VV * i;
-    uint32_t w[4][WV];
+  for (int k = 0; k < KG; ++k) {
+    const char* vs = ring + k * 2 * L::GB + L::GB;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = 2 * j + (k & 1) + 8 * (k >> 1);
-      lds<L::VV>(vs + piece<L::CPR, true>(row, byte >> 4) * 16 + (byte & 15), w[k]);
-    }
+    for (int i = 0; i < L::RB / (8 * L::VV); ++i) {
+      const int byte = L::VV * g + 8 * L::VV * i;
+      uint32_t w[4][WV];
 #pragma unroll
-    for (int x = 0; x < WV; ++x) {
-      if (F8) {
-        // two columns of two keys in a word: (key, key + 1) of one column, then of the next
-        const uint32_t b0 = __byte_perm(w[0][x], w[1][x], 0x5140), b1 = __byte_perm(w[2][x], w[3][x], 0x5140);
-        const uint32_t v[4] = {e4m3_to_f16(b0), e4m3_to_f16(b0 >> 16), e4m3_to_f16(b1), e4m3_to_f16(b1 >> 16)};
-        const int y = (i * EV + 4 * x) / 2;
+      for (int m = 0; m < 4; ++m) {
+        const int row = 2 * j + (m & 1) + 8 * (m >> 1);
+        lds<L::VV>(vs + piece<L::CPR, true>(row, byte >> 4) * 16 + (byte & 15), w[m]);
+      }
 #pragma unroll
-        for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y], v, p[n][0], p[n][1]);
-        if (EV > 2) {
-          const uint32_t c0 = __byte_perm(w[0][x], w[1][x], 0x7362), c1 = __byte_perm(w[2][x], w[3][x], 0x7362);
-          const uint32_t u[4] = {e4m3_to_f16(c0), e4m3_to_f16(c0 >> 16), e4m3_to_f16(c1), e4m3_to_f16(c1 >> 16)};
+      for (int x = 0; x < WV; ++x) {
+        if (F8) {
+          // two columns of two keys in a word: (key, key + 1) of one column, then of the next
+          uint32_t v[4];
+          e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x5140), v[0], v[1]);
+          e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x5140), v[2], v[3]);
+          const int y = (i * EV + 4 * x) / 2;
 #pragma unroll
-          for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y + 1], u, p[n][0], p[n][1]);
+          for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+          if (EV > 2) {
+            e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x7362), v[0], v[1]);
+            e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x7362), v[2], v[3]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y + 1], v, p[k][n][0], p[k][n][1]);
+          }
+        } else {
+          const uint32_t v[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
+                                 __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
+          const int y = (i * EV + 2 * x) / 2;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
         }
-      } else {
-        const uint32_t v[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
-                               __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
-        const int y = (i * EV + 2 * x) / 2;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[n][0], p[n][1]);
       }
     }
   }
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------------------
-// kSplit: the four warps share 8 * NB rows and take 16 of every 64 keys each; otherwise each has 8 * NB rows and takes all keys.
-template <int HD, bool F8, int NB, bool kSplit>
-struct Form {
+template <class F>
+__global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(const Attn a) {
+  constexpr int HD = F::HD, NB = F::NB;
+  constexpr bool F8 = F::F8, kSplit = F::kSplit;
   using L = Layout<HD, F8>;
-  static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
-  // resident CTAs wanted: registers for outputs and queries decide
-  static constexpr int kRegs = NB * (HD / 16 * 6 + 16);
-  static constexpr int kCtas = kRegs <= 80 ? 4 : kRegs <= 112 ? 3 : 2;
-  static constexpr int kRoom = 224 * 1024 / kCtas - 4096, kFit = kRoom / L::STAGE;
-  static constexpr int kStages = kFit < 3 ? 3 : kFit > 6 ? 6 : kFit;
-  static constexpr int kJoin = kSplit ? kWarps * kRows * HD * 4 : 0;
-  static constexpr int kSmem = kStages * L::STAGE > kJoin ? kStages * L::STAGE : kJoin;
-};
-
-template <int HD, bool F8, int NB, bool kSplit>
-__global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_attention_kernel(const Attn a) {
-  using L = Layout<HD, F8>;
-  using F = Form<HD, F8, NB, kSplit>;
-  constexpr int kRows = F::kRows, kStages = F::kStages;
+  constexpr int kRows = F::kRows, kWarps = F::kWarps, kLoads = F::kLoads, kTile = F::kTile, kThreads = F::kThreads;
   extern __shared__ __align__(128) char ring[];
-  __shared__ float2 scales[kStages][kWarps];
+  __shared__ float2 scales[F::kDeep][kWarps * kLoads];
   __shared__ float join_m[kWarps][8 * NB], join_l[kWarps][8 * NB];
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
-  const int page = a.kv.page_size;
-  const int capacity = (int)min((long long)a.kv.table_pitch * page, (long long)INT32_MAX);
-  const Plan plan = make_plan<kRows>(a, capacity);
+  Item it;
+  const Plan plan = make_plan<F>(a, it);
   if (tid == 0) a.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  const uint32_t ring_at = smem_u32(ring);
-  int b = plan.b, mt = plan.mt, head = plan.head, off = plan.off;
-  if (b < 0) {
+  if (it.b < 0) {
     pdl_trigger();
     return;
   }
-  Span s = span_of(a.batch, b, capacity, a.max_new, a.status);
-  for (long long unit = plan.first; unit < plan.last;) {
-    const int rows0 = mt * kRows;
-    const Range range = range_of(s, rows0, kRows, a.group, a.window);
-    const int tiles = range.tiles();
-    const int count = plan.whole ? tiles : (int)min((long long)(tiles - off), plan.last - unit);
-    const int tile0 = range.t0() + off;
+  const uint32_t ring_at = smem_u32(ring);
+  const int warp_rows = kSplit ? 0 : warp * 8 * NB;  // the warp's first row of a tile's
+  RawRows<HD, NB> raw;
+  fetch_queries<HD, F8, NB>(a, it, it.mt * kRows + warp_rows, raw);
 
-    // copies of tile0 + i, i < count: this warp's 16 keys of each.  Where they lie (in 16-byte pieces; all ones: nowhere) and their scales,
-    // of 32 tiles ahead, are in its lanes.
+  Rows<HD, F8, NB> r;
+  for (;;) {
+    const int rows0 = it.mt * kRows + warp_rows, tile0 = it.range.template t0<F>() + it.off;
+    // copies of tile0 + i, i < count: kLoads groups of 16 keys of each by this warp.  Where they lie (in 16-byte pieces; all ones:
+    // nowhere) and their scales, of the next 32 groups, are in its lanes.
+    constexpr int kAhead = 32 / kLoads;  // tiles
     uint32_t my_at = 0xffffffffu;
     float my_k = 1.f, my_v = 1.f;
     auto look_up = [&](int i) {
-      const int key = (tile0 + i + lane) * kTile + warp * kGroup;
+      const int key = (tile0 + i + lane / kLoads) * kTile + (warp * kLoads + lane % kLoads) * kGroup;
       my_at = 0xffffffffu;
       my_k = my_v = 1.f;
-      if (i + lane < count && key < range.hi && key + kGroup > range.lo) {
-        const int slot = key / page, p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
+      if (i + lane / kLoads < it.count && key < it.range.hi && key + kGroup > it.range.lo) {
+        const int slot = a.by_page(key), p = a.kv.table[(size_t)it.b * a.kv.table_pitch + slot];
         if (p < 0 || p >= a.kv.n_pages) {
           atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
         } else {
-          my_at = (uint32_t)(((unsigned long long)p * a.kv.page_stride + ((size_t)head * page + key - slot * page) * HD) * L::ES >> 4);
+          my_at = (uint32_t)(((unsigned long long)p * a.kv.page_stride +
+                              ((size_t)it.head * a.kv.page_size + key - slot * a.kv.page_size) * HD) * L::ES >> 4);
           if (F8) {
-            my_k = a.kv.k_scale[(size_t)p * a.kv.kv_heads + head];
-            my_v = a.kv.v_scale[(size_t)p * a.kv.kv_heads + head];
+            my_k = a.kv.k_scale[(size_t)p * a.kv.kv_heads + it.head];
+            my_v = a.kv.v_scale[(size_t)p * a.kv.kv_heads + it.head];
           }
         }
       }
     };
     int to_stage = 0, from_stage = 0;
     auto copy = [&](int i) {
-      if (i < count) {
-        if ((i & 31) == 0) look_up(i);
-        const uint32_t at = __shfl_sync(0xffffffffu, my_at, i & 31);
-        const int key0 = (tile0 + i) * kTile + warp * kGroup;
-        if (F8) {
-          const float ks = __shfl_sync(0xffffffffu, my_k, i & 31), vs = __shfl_sync(0xffffffffu, my_v, i & 31);
-          if (lane == 0) scales[to_stage][warp] = make_float2(ks, vs);
-        }
-        const uint32_t to = ring_at + to_stage * L::STAGE + warp * 2 * L::GB;
-        const char *k = reinterpret_cast<const char*>(a.kv.k) + (size_t)at * 16, *v = reinterpret_cast<const char*>(a.kv.v) + (size_t)at * 16;
-        if (key0 >= range.lo && key0 + kGroup <= range.hi && at != 0xffffffffu) {
+      if (i < it.count) {
+        if (i % kAhead == 0) look_up(i);
+        const char* none = reinterpret_cast<const char*>(a.kv.k);
 #pragma unroll
-          for (int c0 = 0; c0 < L::GB / 16; c0 += 32) {
-            const int c = c0 + lane;
-            if ((L::GB / 16) % 32 == 0 || c < L::GB / 16) {
+        for (int n = 0; n < kLoads; ++n) {
+          const uint32_t at = __shfl_sync(0xffffffffu, my_at, i % kAhead * kLoads + n);
+          const int key0 = (tile0 + i) * kTile + (warp * kLoads + n) * kGroup;
+          const uint32_t to = ring_at + to_stage * F::kStage + (warp * kLoads + n) * 2 * L::GB;
+          const char *k = none + (size_t)at * 16, *v = reinterpret_cast<const char*>(a.kv.v) + (size_t)at * 16;
+          if (key0 >= it.range.lo && key0 + kGroup <= it.range.hi && at != 0xffffffffu) {
+#pragma unroll
+            for (int c0 = 0; c0 < L::GB / 16; c0 += 32) {
+              const int c = c0 + lane;
+              if ((L::GB / 16) % 32 == 0 || c < L::GB / 16) {
+                const int row = c / L::CPR, in_row = c % L::CPR;
+                copy_16(to + piece<L::CPR, false>(row, in_row) * 16, k + c * 16, true);
+                copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, v + c * 16, true);
+              }
+            }
+          } else {
+            // rows that no query sees are filled with zeros: whatever lies there must not count
+            const int lo = it.range.lo - key0, hi = at == 0xffffffffu ? 0 : it.range.hi - key0;
+#pragma unroll 1
+            for (int c = lane; c < L::GB / 16; c += 32) {
               const int row = c / L::CPR, in_row = c % L::CPR;
-              copy_16(to + piece<L::CPR, false>(row, in_row) * 16, k + c * 16, true);
-              copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, v + c * 16, true);
+              const bool take = row >= lo && row < hi;
+              copy_16(to + piece<L::CPR, false>(row, in_row) * 16, take ? k + c * 16 : none, take);
+              copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, take ? v + c * 16 : none, take);
             }
           }
-        } else {
-          // rows that no query sees are filled with zeros: whatever lies there must not count
-          const int lo = range.lo - key0, hi = at == 0xffffffffu ? 0 : range.hi - key0;
-#pragma unroll 1
-          for (int c = lane; c < L::GB / 16; c += 32) {
-            const int row = c / L::CPR, in_row = c % L::CPR;
-            const bool take = row >= lo && row < hi;
-            copy_16(to + piece<L::CPR, false>(row, in_row) * 16, take ? k + c * 16 : reinterpret_cast<const char*>(a.kv.k), take);
-            copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, take ? v + c * 16 : reinterpret_cast<const char*>(a.kv.v), take);
-          }
         }
-        if (++to_stage == kStages) to_stage = 0;
+        if (++to_stage == a.stages) to_stage = 0;
       }
       copy_commit();
     };
+    // scales follow their copies, as they arrive later than the pages' numbers
+    int scaled = 0, scale_stage = 0;
+    auto put_scales = [&]() {
+      if (F8 && scaled < it.count) {
+        if (lane / kLoads == scaled % kAhead) scales[scale_stage][warp * kLoads + lane % kLoads] = make_float2(my_k, my_v);
+        ++scaled;
+        if (++scale_stage == a.stages) scale_stage = 0;
+      }
+    };
 #pragma unroll 1
-    for (int i = 0; i < kStages - 1; ++i) copy(i);
-
-    Rows<HD, F8, NB> r;
-    const int my_rows0 = rows0 + (kSplit ? 0 : warp * 8 * NB);
-    load_queries<HD, F8, NB>(a, s, my_rows0, head, r);
+    for (int i = 0; i < a.stages - 1; ++i) copy(i);
+#pragma unroll 1
+    for (int i = 0; i < a.stages - 1; ++i) put_scales();
+    begin_rows<HD, F8, NB>(a, it, rows0, raw, r);
     // positions of the warp's first and last row
-    const bool any_row = my_rows0 < s.n * a.group;
-    const int p_first = s.pos + my_rows0 / a.group, p_last = s.pos + min(s.n - 1, (my_rows0 + 8 * NB - 1) / a.group);
-
+    const bool any_row = kSplit || rows0 < it.s.n * a.group;
+    const int p_first = it.s.pos + (kSplit ? 0 : a.by_group(rows0));
+    const int p_last = it.s.pos + (kSplit ? it.s.n - 1 : min(it.s.n - 1, a.by_group(rows0 + 8 * NB - 1)));
 #pragma unroll 1
-    for (int i = 0; i < count; ++i) {
-      copy_wait<kStages - 2>();
+    for (int i = 0; i < it.count; ++i) {
+      if (a.stages == F::kStages) copy_wait<F::kStages - 2>();
+      else copy_wait<F::kDeep - 2>();
       if (kSplit) __syncwarp();
       else __syncthreads();
-      copy(i + kStages - 1);
-      const char* at = ring + from_stage * L::STAGE;
+      copy(i + a.stages - 1);
+      put_scales();
+      const char* at = ring + from_stage * F::kStage;
+      constexpr int KG = F::kGroups;
+      const int key_tile = (tile0 + i) * kTile;
 #pragma unroll 1
-      for (int w = kSplit ? warp : 0; w < (kSplit ? warp + 1 : kWarps); ++w) {
-        const int key0 = (tile0 + i) * kTile + w * kGroup;
-        if (!any_row || key0 > p_last || (a.window && key0 + kGroup - 1 <= p_first - a.window)) continue;
-        const bool checked = key0 + kGroup - 1 > p_first || (a.window && key0 <= p_last - a.window);
-        const float2 scale = F8 ? scales[from_stage][w] : make_float2(1.f, 1.f);
-        keys_16<HD, F8, NB>(at + w * 2 * L::GB, at + w * 2 * L::GB + L::GB, key0, checked, a.window, scale.x, scale.y, r);
+      for (int w = kSplit ? warp * kLoads : 0; w < (kSplit ? (warp + 1) * kLoads : kWarps * kLoads); w += KG) {
+        const int key0 = key_tile + w * kGroup;
+        if (!any_row || key0 > p_last || (a.window && key0 + KG * kGroup - 1 <= p_first - a.window)) continue;
+        const bool checked = key0 + KG * kGroup - 1 > p_first || (a.window && key0 <= p_last - a.window);
+        take_keys<HD, F8, NB, KG>(at + w * 2 * L::GB, &scales[from_stage][w], key0, checked, a.window, r);
       }
-      if (++from_stage == kStages) from_stage = 0;
+      if (++from_stage == a.stages) from_stage = 0;
     }
     copy_wait<0>();
 
-    // the item's end: rows' sums over their threads, and over the warps where those took different keys
-    const bool begins = off == 0, ends = off + count == tiles, complete = begins && ends;
+    // the item's end; the queries of the next one are fetched meanwhile
+    const Item done = it;
+    const bool another = next_item<F>(a, plan, it);
+    if (another) fetch_queries<HD, F8, NB>(a, it, it.mt * kRows + warp_rows, raw);
+    // rows' sums over their threads, and over the warps where those took different keys
+    const bool begins = done.off == 0, ends = done.off + done.count == done.tiles, complete = begins && ends;
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
     float unit_o = 1.f;
     if (F8) unit_o = r.v_ref * (1.f / kPScale);
@@ -623,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_
         for (int h = 0; h < 2; ++h) {
           const int row = 8 * n + 2 * j + h;
           if (g == 0) {
-            join_m[warp][row] = r.m[n][h];
+            join_m[warp][row] = r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h];
             join_l[warp][row] = r.l[n][h];
           }
 #pragma unroll
@@ -632,9 +815,9 @@ __global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_
                 make_float2(r.o[n][y][h] * unit_o, r.o[n][y][2 + h] * unit_o);
         }
       __syncthreads();
-      const int n_rows = min(kRows, s.n * a.group - rows0);
-      for (int i = tid; i < n_rows * (HD / 4); i += kThreads) {
-        const int row = i / (HD / 4), col = i % (HD / 4) * 4;
+      const int n_rows = done.s.n * a.group;
+      for (int k = tid; k < n_rows * (HD / 4); k += kThreads) {
+        const int row = k / (HD / 4), col = k % (HD / 4) * 4;
         float top = join_m[0][row];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w][row]);
@@ -644,14 +827,13 @@ __global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_
         for (int w = 0; w < kWarps; ++w) {
           const float by = exp2_fast(join_m[w][row] - base);
           const float4 v = *reinterpret_cast<const float4*>(o_at + (w * kRows + row) * HD + col);
-          if (join_m[w][row] == -INFINITY && join_l[w][row] == 0.f) continue;  // saw nothing
           l += join_l[w][row] * by;
           o[0] += v.x * by; o[1] += v.y * by; o[2] += v.z * by; o[3] += v.w * by;
         }
         if (complete) {
           const float by = l == 0.f ? 0.f : 1.f / l;
-          const int t = (rows0 + row) / a.group, hd = (rows0 + row) % a.group;
-          *reinterpret_cast<uint2*>(a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(head * a.group + hd) * HD + col) =
+          const int t = a.by_group(row), hd = row - t * a.group;
+          *reinterpret_cast<uint2*>(a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD + col) =
               make_uint2(pack<false>(o[0] * by, o[1] * by), pack<false>(o[2] * by, o[3] * by));
         } else {
           *reinterpret_cast<float4*>(a.part + ((size_t)slot * kRows + row) * HD + col) = make_float4(o[0], o[1], o[2], o[3]);
@@ -663,13 +845,13 @@ __global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = warp * 8 * NB + 8 * n + 2 * j + h, at = rows0 + row;
-          if (at >= s.n * a.group) continue;
+          const int row = warp_rows + 8 * n + 2 * j + h, at = done.mt * kRows + row;
+          if (at >= done.s.n * a.group) continue;
           const float by = complete ? (r.l[n][h] == 0.f ? 0.f : unit_o / r.l[n][h]) : unit_o;
-          const int t = at / a.group, hd = at % a.group;
-          bf16* out = a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(head * a.group + hd) * HD;
+          const int t = a.by_group(at), hd = at - t * a.group;
+          bf16* out = a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD;
           float* part = a.part + ((size_t)slot * kRows + row) * HD;
-          if (!complete && g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.m[n][h], r.l[n][h]);
+          if (!complete && g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h], r.l[n][h]);
 #pragma unroll
           for (int y = 0; y < HD / 16; ++y) {
             const int col = column<HD, F8>(2 * y, g);
@@ -681,117 +863,149 @@ __global__ void __launch_bounds__(kThreads, Form<HD, F8, NB, kSplit>::kCtas) kv_
     }
     if (!complete && begins && tid == 0) {
       // parts: this CTA's and one of each of the next ones until the item ends
-      const long long end = unit + tiles;
-      a.head[blockIdx.x] = make_int4(b, mt, head, (int)((end - 1) / plan.share - blockIdx.x) + 1);
+      const uint32_t last = plan.cut == kPieces ? blockIdx.x + (uint32_t)(done.tiles - 1) / (uint32_t)plan.share
+                                                : (uint32_t)(done.unit + done.tiles - 1) / (uint32_t)plan.share;
+      a.head[blockIdx.x] = make_int4(done.b, done.mt, done.head, (int)(last - blockIdx.x) + 1);
     }
+    if (!another) break;
     __syncthreads();  // the ring and the join buffers are free again
-    unit += plan.whole ? 1 : count;
-    off = 0;
-    if (unit < plan.last && ++head == a.kv.kv_heads) {
-      head = 0;
-      ++mt;
-      while (mt * kRows >= s.n * a.group) {
-        mt = 0;
-        s = span_of(a.batch, ++b, capacity, a.max_new, a.status);
-      }
-    }
   }
-  pdl_trigger();
+  pdl_trigger();  // not earlier: the next kernel's CTAs would take the room of this one's second half
 }
 
-// Joins the parts of shared items: a block for each CTA of the first kernel and row of a tile.
+// Joins the parts of shared items: a block for each CTA of the first kernel and row of a tile.  Factors of all parts first, so that the
+// parts themselves are read without waiting for one another.
+constexpr int kJoinThreads = 256, kMostParts = 1024;
+
 template <int HD, int kRows>
-__global__ void __launch_bounds__(kThreads) kv_join_kernel(const Attn a) {
-  pdl_trigger();
-  pdl_wait();
-  const int4 item = a.head[blockIdx.x];
-  if (item.x < 0) return;
+__device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int row) {
   const Span s = span_of(a.batch, item.x, INT32_MAX, INT32_MAX, a.status);
-  const int row = blockIdx.y, at = item.y * kRows + row, parts = item.w, tid = threadIdx.x;
+  const int at = item.y * kRows + row, parts = item.w, tid = threadIdx.x, warp = tid >> 5;
   if (at >= s.n * a.group) return;
   // part i: the first CTA's second slot, then the first slot of each
-  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * kRows + row; };
-  constexpr int lanes = HD / 4, teams = kThreads / lanes;  // a team goes over every teams-th part
+  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row; };
+  constexpr int lanes = HD / 4, teams = kJoinThreads / lanes, kMine = kMostParts / kJoinThreads;  // a team takes every teams-th part
+  __shared__ float factor[kMostParts];
+  __shared__ float most[kJoinThreads / 32], total[kJoinThreads / 32];
   __shared__ float4 sums[teams][lanes];
-  __shared__ float2 stats[teams];
   const int team = tid / lanes, lane = tid % lanes;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 st[kMine];
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int i = tid + k * kJoinThreads;
+    st[k] = i < parts ? a.stats[slot(i)] : make_float2(-INFINITY, 0.f);
+  }
+  constexpr int kEarly = 8;  // parts that are on their way before the factors are known
+  float4 early[kEarly];
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = team + k * teams;
+    early[k] = team < teams && i < parts ? *reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) m = fmaxf(m, st[k].x);
+  m = warp_max(m);
+  if ((tid & 31) == 0) most[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, most[i]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int i = tid + k * kJoinThreads;
+    const float f = exp2_fast(st[k].x - base);
+    if (i < parts) factor[i] = f;
+    l += st[k].y * f;
+  }
+  l = warp_sum(l);
+  if ((tid & 31) == 0) total[warp] = l;
+  __syncthreads();
   if (team < teams) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, float f) {
+      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    };
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+      if (team + k * teams < parts) add(early[k], factor[team + k * teams]);
 #pragma unroll 4
-    for (int i = team; i < parts; i += teams) {
-      const float2 st = a.stats[slot(i)];
-      const float4 v = *reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4);
-      if (st.x == -INFINITY && st.y == 0.f) continue;
-      const float top = fmaxf(m, st.x), base = top == -INFINITY ? 0.f : top;
-      const float f = exp2_fast(m - base), by = exp2_fast(st.x - base);
-      m = top;
-      l = l * f + st.y * by;
-      o.x = o.x * f + v.x * by; o.y = o.y * f + v.y * by; o.z = o.z * f + v.z * by; o.w = o.w * f + v.w * by;
-    }
+    for (int i = team + kEarly * teams; i < parts; i += teams)
+      add(*reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4), factor[i]);
     sums[team][lane] = o;
-    if (lane == 0) stats[team] = make_float2(m, l);
   }
   __syncthreads();
   if (tid >= lanes) return;
-  m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < teams; ++i) m = fmaxf(m, stats[i].x);
-  const float base = m == -INFINITY ? 0.f : m;
   l = 0.f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < teams; ++i) {
-    if (stats[i].x == -INFINITY && stats[i].y == 0.f) continue;
-    const float by = exp2_fast(stats[i].x - base);
+  for (int i = 0; i < kJoinThreads / 32; ++i) l += total[i];
+  float4 o = sums[0][tid];
+  for (int i = 1; i < min(teams, parts); ++i) {
     const float4 v = sums[i][tid];
-    l += stats[i].y * by;
-    o.x += v.x * by; o.y += v.y * by; o.z += v.z * by; o.w += v.w * by;
+    o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
   }
   const float by = l == 0.f ? 0.f : 1.f / l;
-  const int t = at / a.group, hd = at % a.group;
+  const int t = a.by_group(at), hd = at - t * a.group;
   *reinterpret_cast<uint2*>(a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(item.z * a.group + hd) * HD + tid * 4) =
       make_uint2(pack<false>(o.x * by, o.y * by), pack<false>(o.z * by, o.w * by));
 }
 
-// CTAs of a wave: bounded so that the workspace's size is known without asking for the occupancy.
-constexpr int kMostPerSm = 4;
+// One row of one shared item a time.  Most CTAs of the first kernel begin none: 32 of them are looked at together.
+template <int HD, int kRows>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int ctas, int rows) {
+  pdl_trigger();
+  pdl_wait();
+  // this block's tasks: blockIdx.x, + gridDim.x, ...; task t is row t % rows of CTA t / rows
+  const int lane = threadIdx.x & 31, tasks = ctas * rows;
+  for (int t0 = blockIdx.x; t0 < tasks; t0 += 32 * gridDim.x) {
+    const int mine = t0 + lane * (int)gridDim.x;
+    const int4 item = mine < tasks ? a.head[mine / rows] : make_int4(-1, 0, 0, 0);
+    for (uint32_t left = __ballot_sync(0xffffffffu, item.x >= 0); left; left &= left - 1) {
+      const int from = __ffs(left) - 1, t = t0 + from * (int)gridDim.x;
+      const int4 one = make_int4(__shfl_sync(0xffffffffu, item.x, from), __shfl_sync(0xffffffffu, item.y, from),
+                                 __shfl_sync(0xffffffffu, item.z, from), __shfl_sync(0xffffffffu, item.w, from));
+      join_row<HD, kRows>(a, t / rows, one, t % rows);
+      __syncthreads();
+    }
+  }
+}
 
-template <int HD, bool F8, int NB, bool kSplit>
+template <class F>
 cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
-  using F = Form<HD, F8, NB, kSplit>;
-  constexpr int kRows = F::kRows, most = F::kCtas;
-  static_assert(most <= kMostPerSm, "the workspace is sized for this many");
+  constexpr int kRows = F::kRows, kTile = F::kTile, most = F::kCtas;
+  static_assert(most <= 2 && kRows <= (F::HD <= 64 ? 128 : 64), "the workspace is sized for these");
   static unsigned long long opted = 0;
-  auto kernel = kv_attention_kernel<HD, F8, NB, kSplit>;
-  if (!smem_opt_in(kernel, F::kSmem, opted)) return cudaGetLastError();
-  // no more CTAs than there can be units: items, or pieces of kLeast tiles of them
-  const long long capacity = (long long)a.kv.table_pitch * a.kv.page_size;
-  const long long longest = a.window ? min(capacity, (long long)a.window + (kRows - 1) / a.group + kTile) : capacity;
+  auto kernel = kv_attention_kernel<F>;
+  if (!smem_opt_in(kernel, F::kDeep * F::kStage, opted)) return cudaGetLastError();
+  // no more CTAs than there can be units: items, or shares of F::kLeast tiles of them
+  const long long longest = a.window ? min((long long)a.capacity, (long long)a.window + (kRows - 1) / a.group + kTile) : a.capacity;
   const long long items = (((long long)a.batch.n_tokens * a.group) / kRows + a.batch.n_seq) * a.kv.kv_heads;
-  const long long pieces = ((longest + kTile - 1) / kTile + 1 + kLeast - 1) / kLeast;
-  const bool may_share = (longest + kTile - 1) / kTile > kLeast;
-  const int ctas = (int)min((long long)sms * most, may_share ? items * pieces : items);
+  const long long tiles = (longest + kTile - 1) / kTile + (a.window ? 1 : 0);
+  if (items * tiles > INT32_MAX) return cudaErrorInvalidValue;
+  const bool may_share = tiles > F::kAlone;
+  const int ctas = (int)min(min((long long)sms * most, (long long)kMostParts), may_share ? items * (tiles / F::kLeast + 2) : items);
+  // a CTA that has an SM to itself may fetch further ahead
+  a.stages = ctas <= sms ? F::kDeep : F::kStages;
   char* at = reinterpret_cast<char*>(workspace);
   a.head = reinterpret_cast<int4*>(at);
   at += sizeof(int4) * (size_t)sms * most;
   a.stats = reinterpret_cast<float2*>(at);
   at += sizeof(float2) * 2 * (size_t)sms * most * kRows;
   a.part = reinterpret_cast<float*>(at);
-  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), F::kSmem, s, a);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(F::kThreads), a.stages * F::kStage, s, a);
   if (e != cudaSuccess || !may_share) return e;
   const int rows = (int)min((long long)kRows, (long long)a.max_new * a.group);
-  return launch_pdl(kv_join_kernel<HD, kRows>, dim3((unsigned)ctas, (unsigned)rows), dim3(kThreads), 0, s, a);
+  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, 4ll * sms)), dim3(kJoinThreads), 0, s, a, ctas, rows);
 }
 
 // Rows of one KV head at most: which form.
 template <int HD, bool F8>
 cudaError_t run_rows(const Attn& a, int sms, void* workspace, cudaStream_t s) {
-  constexpr int kMany = HD <= 64 ? 4 : 2;
   const long long rows = (long long)a.max_new * a.group;
-  if (rows <= 8) return run<HD, F8, 1, true>(a, sms, workspace, s);
-  if (rows <= 16) return run<HD, F8, 2, true>(a, sms, workspace, s);
-  return run<HD, F8, kMany, false>(a, sms, workspace, s);
+  if (rows <= 8) return run<Form<HD, F8, 1, true>>(a, sms, workspace, s);
+  if (rows <= 16) return run<Form<HD, F8, 2, true>>(a, sms, workspace, s);
+  return run<Form<HD, F8, HD <= 64 ? 4 : 2, false>>(a, sms, workspace, s);
 }
 template <int HD>
 cudaError_t run_hd(const Attn& a, int sms, void* workspace, cudaStream_t s) {
@@ -807,13 +1021,7 @@ static size_t workspace_of(int sms) {
   auto bytes = [&](size_t per_sm, size_t rows) {
     return sms * per_sm * (sizeof(int4) + 2 * rows * (sizeof(float2) + sizeof(float) * HD));
   };
-  using A = Form<HD, false, 1, true>;
-  using B = Form<HD, false, 2, true>;
-  using C = Form<HD, false, HD <= 64 ? 4 : 2, false>;
-  size_t most = bytes(A::kCtas, A::kRows);
-  if (bytes(B::kCtas, B::kRows) > most) most = bytes(B::kCtas, B::kRows);
-  if (bytes(C::kCtas, C::kRows) > most) most = bytes(C::kCtas, C::kRows);
-  return most;
+  return bytes(2, HD <= 64 ? 128 : 64);  // the form of most rows, and no form has more CTAs
 }
 size_t kv_attention_workspace(int sms, int hd) {  // the same for both types of cache
   switch (hd) {
@@ -837,6 +1045,9 @@ cudaError_t kv_attention(const PagedKv& kv, const Batch& batch, int heads, const
   a.batch = batch;
   a.q = q; a.out = out; a.ld_q = ld_q; a.ld_out = ld_out;
   a.group = heads / kv.kv_heads;
+  a.capacity = (int)min((long long)kv.table_pitch * kv.page_size, (long long)INT32_MAX - kv.page_size);
+  a.by_group = Div(a.group);
+  a.by_page = Div(kv.page_size);
   a.max_new = max_new;
   a.window = window;
   a.scale_log2 = (scale == 0.f ? (float)(1.0 / sqrt((double)kv.head_dim)) : scale) * 1.4426950408889634f;
