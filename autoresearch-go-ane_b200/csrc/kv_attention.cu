@@ -73,7 +73,7 @@ struct Form {
   using L = Layout<HD, F8>;
   static constexpr int kGroups = kSplit ? (L::RB <= 64 && NB == 1 ? 2 : 1) : 2;
   // groups of 16 keys of a tile that a warp fetches; the ring has to hold the outputs of kSplit's warps
-  static constexpr int kLoads = kSplit ? kGroups : 1;
+  static constexpr int kLoads = kSplit || L::RB <= 128 ? kGroups : 1;
   static constexpr int kThreads = 32 * kWarps, kTile = kGroup * kWarps * kLoads;
   static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
   static constexpr int kStage = kWarps * kLoads * 2 * L::GB;
@@ -86,17 +86,27 @@ struct Form {
   static_assert(!kSplit || kWarps * kRows * HD * 4 <= 3 * kStage, "the warps' outputs are joined in the ring");
   // Tiles of an item that are not worth sharing (joining parts takes a second kernel), and the least share of one that is shared.
   static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile;
-  static constexpr int kRestart = kSplit ? 768 / kTile : 1;  // what another item costs a CTA, in tiles
+  static constexpr int kRestart = 768 / kTile;  // what another item costs a CTA, in tiles
 };
 
-// Where 16-byte piece c of a row lies within 16 rows, so that the threads of a fragment load find it in different banks: a thread
-// (g, j) reads row g of K at pieces j.. and row 2 j (+ 1, 8, 9) of V at pieces g...
-template <int CPR, bool V>
+// Where 16-byte piece c of a row lies within 16 rows, so that what is read together lies in different banks.  bf16: the same piece of eight
+// rows (ldmatrix).  8 bits: a thread (g, j) reads row g of K at pieces j.. and row 2 j (+ 1, 8, 9) of V at pieces g...
+template <int CPR, bool F8, bool V>
 __device__ __forceinline__ int piece(int row, int c) {
+  if (!F8) {
+    if (CPR % 8 == 0) return row * CPR + (c ^ (row & 7));
+    if (CPR % 4 == 0) return row * CPR + (c ^ (row >> 1 & 3));
+    return row * CPR + (c ^ (row >> 2 & 1));
+  }
   if (CPR % 8 == 0) return row * CPR + (c ^ (V ? row & 7 : (row & 1) << 2));
   if (CPR == 4) return (row >> 1) * 8 + ((((row & 1) << 2) | c) ^ ((row >> 1 & 3) << 1));
   if (CPR == 2) return (row >> 2) * 8 + ((((row & 3) << 1) | c) ^ ((row >> 2 & 1) << 1));
   return row * CPR + c;
+}
+template <bool kTrans>
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&a)[4]) {
+  if (kTrans) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at));
+  else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at));
 }
 
 template <bool F8>
@@ -274,7 +284,7 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
     const int even = max(quotient_up(tiles, ctas), F::kLeast);
     // at most tiles / share + items pieces
     const int pieces = items < ctas ? max(quotient_up(tiles, ctas - items), even) : INT32_MAX;
-    p.cut = pieces <= even + F::kRestart ? kPieces : kEven;
+    p.cut = F::kSplit && pieces <= even + F::kRestart ? kPieces : kEven;
     p.share = p.cut == kPieces ? pieces : even;
   }
   auto weight = [&](int t) { return p.cut == kWhole ? 1 : p.cut == kPieces ? quotient_up(t, p.share) : t; };
@@ -358,9 +368,11 @@ __device__ __forceinline__ void fetch_queries(const Attn& a, const Item& it, int
     const bf16* q = a.q + (size_t)(it.s.row + t) * a.ld_q + (size_t)(it.head * a.group + hd) * HD;
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) {
-      // the four elements that word i (8 bits), or words 2 i and 2 i + 1, of the thread's bytes of a K row meet
-      const int word = F8 ? i : 2 * i, at = (L::VK * j + word / (L::VK / 4) * 4 * L::VK + word % (L::VK / 4) * 4) / L::ES;
-      raw.w[n][i] = there ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0, 0);
+      // 8 bits: the four elements that word i of the thread's bytes of a K row meets
+      const int at = F8 ? L::VK * j + i / (L::VK / 4) * 4 * L::VK + i % (L::VK / 4) * 4 : 16 * i + 2 * j;
+      if (!there) raw.w[n][i] = make_uint2(0, 0);
+      else if (F8) raw.w[n][i] = *reinterpret_cast<const uint2*>(q + at);
+      else raw.w[n][i] = make_uint2(*reinterpret_cast<const uint32_t*>(q + at), *reinterpret_cast<const uint32_t*>(q + at + 8));
     }
   }
 }
@@ -422,12 +434,12 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w >> 16 & 0x7f80u) == 0x7f80u;
 }
 
-// Column of the output that group x of a thread's bytes of V rows (element x) stands for in the threads with this g.
+// Column of the output that element x of a thread's products with V stands for in the threads with this g.
 template <int HD, bool F8>
 __device__ __forceinline__ int column(int x, int g) {
   using L = Layout<HD, F8>;
   constexpr int EV = L::VV / L::ES;
-  return x / EV * 8 * EV + g * EV + x % EV;
+  return F8 ? x / EV * 8 * EV + g * EV + x % EV : 8 * x + g;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 matrix of 16-bit values
   uint32_t r;
@@ -453,25 +465,35 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[k][n][i] = even[n][i] = 0.f;
+    auto products = [&](const uint32_t (&a)[4], int step) {
 #pragma unroll
-    for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
-      const int byte = L::VK * j + 4 * L::VK * i;
-      uint32_t u[L::VK / 4], w[L::VK / 4];  // of keys g and g + 8
-      lds<L::VK>(ks + piece<L::CPR, false>(g, byte >> 4) * 16 + (byte & 15), u);
-      lds<L::VK>(ks + piece<L::CPR, false>(8 + g, byte >> 4) * 16 + (byte & 15), w);
+      for (int n = 0; n < NB; ++n) {
+        if (kChains == 2 && step % 2 == 0) mma<F8>(even[n], a, r.q[n][step][0], r.q[n][step][1]);
+        else mma<F8>(s[k][n], a, r.q[n][step][0], r.q[n][step][1]);
+      }
+    };
+    if (F8) {
 #pragma unroll
-      for (int x = 0; x < L::VK / 4; x += F8 ? 1 : 2) {
-        uint32_t a[4] = {u[x], w[x], u[x + !F8], w[x + !F8]};
-        if (F8) {
+      for (int i = 0; i < L::RB / (4 * L::VK); ++i) {
+        const int byte = L::VK * j + 4 * L::VK * i;
+        uint32_t u[L::VK / 4], w[L::VK / 4];  // of keys g and g + 8
+        lds<L::VK>(ks + piece<L::CPR, F8, false>(g, byte >> 4) * 16 + (byte & 15), u);
+        lds<L::VK>(ks + piece<L::CPR, F8, false>(8 + g, byte >> 4) * 16 + (byte & 15), w);
+#pragma unroll
+        for (int x = 0; x < L::VK / 4; ++x) {
+          uint32_t a[4];
           e4m3_to_f16(u[x], a[0], a[2]);
           e4m3_to_f16(w[x], a[1], a[3]);
+          products(a, i * (L::VK / 4) + x);
         }
-        const int step = F8 ? i * (L::VK / 4) + x : (i * (L::VK / 4) + x) / 2;
+      }
+    } else {
+      const uint32_t at = smem_u32(ks);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          if (kChains == 2 && step % 2 == 0) mma<F8>(even[n], a, r.q[n][step][0], r.q[n][step][1]);
-          else mma<F8>(s[k][n], a, r.q[n][step][0], r.q[n][step][1]);
-        }
+      for (int i = 0; i < HD / 16; ++i) {
+        uint32_t a[4];
+        load_matrices<false>(at + piece<L::CPR, F8, false>(lane & 15, 2 * i + (lane >> 4)) * 16, a);
+        products(a, i);
       }
     }
     if (kChains == 2) {
@@ -600,7 +622,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
 #pragma unroll
             for (int x = 0; x < HD / 8; ++x) {
               const int byte = column<HD, F8>(x, g) * L::ES;
-              const char* at = vs + piece<L::CPR, true>(key, byte >> 4) * 16 + (byte & 15);
+              const char* at = vs + piece<L::CPR, F8, true>(key, byte >> 4) * 16 + (byte & 15);
               const float v = F8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*reinterpret_cast<const unsigned char*>(at), __NV_E4M3)))
                                  : __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(at) << 16);
               if (see0) r.o[n][x >> 1][2 * (x & 1)] += w0 * v;
@@ -616,37 +638,39 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
 #pragma unroll
   for (int k = 0; k < KG; ++k) {
     const char* vs = ring + k * 2 * L::GB + L::GB;
+    if (!F8) {
+      const uint32_t at = smem_u32(vs);
 #pragma unroll
-    for (int i = 0; i < L::RB / (8 * L::VV); ++i) {
+      for (int y = 0; y < HD / 16; ++y) {
+        uint32_t v[4];
+        load_matrices<true>(at + piece<L::CPR, F8, true>((lane & 7) + (lane >> 4) * 8, 2 * y + (lane >> 3 & 1)) * 16, v);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < (F8 ? L::RB / (8 * L::VV) : 0); ++i) {
       const int byte = L::VV * g + 8 * L::VV * i;
       uint32_t w[4][WV];
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         const int row = 2 * j + (m & 1) + 8 * (m >> 1);
-        lds<L::VV>(vs + piece<L::CPR, true>(row, byte >> 4) * 16 + (byte & 15), w[m]);
+        lds<L::VV>(vs + piece<L::CPR, F8, true>(row, byte >> 4) * 16 + (byte & 15), w[m]);
       }
 #pragma unroll
       for (int x = 0; x < WV; ++x) {
-        if (F8) {
-          // two columns of two keys in a word: (key, key + 1) of one column, then of the next
-          uint32_t v[4];
-          e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x5140), v[0], v[1]);
-          e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x5140), v[2], v[3]);
-          const int y = (i * EV + 4 * x) / 2;
+        // two columns of two keys in a word: (key, key + 1) of one column, then of the next
+        uint32_t v[4];
+        e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x5140), v[0], v[1]);
+        e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x5140), v[2], v[3]);
+        const int y = (i * EV + 4 * x) / 2;
 #pragma unroll
-          for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
-          if (EV > 2) {
-            e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x7362), v[0], v[1]);
-            e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x7362), v[2], v[3]);
+        for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+        if (EV > 2) {
+          e4m3_to_f16(__byte_perm(w[0][x], w[1][x], 0x7362), v[0], v[1]);
+          e4m3_to_f16(__byte_perm(w[2][x], w[3][x], 0x7362), v[2], v[3]);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y + 1], v, p[k][n][0], p[k][n][1]);
-          }
-        } else {
-          const uint32_t v[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
-                                 __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
-          const int y = (i * EV + 2 * x) / 2;
-#pragma unroll
-          for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+          for (int n = 0; n < NB; ++n) mma<true>(r.o[n][y + (EV > 2)], v, p[k][n][0], p[k][n][1]);
         }
       }
     }
@@ -684,11 +708,11 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
     // nowhere) and their scales, of the next 32 groups, are in its lanes.
     constexpr int kAhead = 32 / kLoads;  // tiles
     uint32_t my_at = 0xffffffffu;
-    float my_k = 1.f, my_v = 1.f;
+    float my_k = 0.f, my_v = 0.f;
     auto look_up = [&](int i) {
       const int key = (tile0 + i + lane / kLoads) * kTile + (warp * kLoads + lane % kLoads) * kGroup;
       my_at = 0xffffffffu;
-      my_k = my_v = 1.f;
+      my_k = my_v = 0.f;
       if (i + lane / kLoads < it.count && key < it.range.hi && key + kGroup > it.range.lo) {
         const int slot = a.by_page(key), p = a.kv.table[(size_t)it.b * a.kv.table_pitch + slot];
         if (p < 0 || p >= a.kv.n_pages) {
@@ -720,8 +744,8 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
               const int c = c0 + lane;
               if ((L::GB / 16) % 32 == 0 || c < L::GB / 16) {
                 const int row = c / L::CPR, in_row = c % L::CPR;
-                copy_16(to + piece<L::CPR, false>(row, in_row) * 16, k + c * 16, true);
-                copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, v + c * 16, true);
+                copy_16(to + piece<L::CPR, F8, false>(row, in_row) * 16, k + c * 16, true);
+                copy_16(to + L::GB + piece<L::CPR, F8, true>(row, in_row) * 16, v + c * 16, true);
               }
             }
           } else {
@@ -731,8 +755,8 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
             for (int c = lane; c < L::GB / 16; c += 32) {
               const int row = c / L::CPR, in_row = c % L::CPR;
               const bool take = row >= lo && row < hi;
-              copy_16(to + piece<L::CPR, false>(row, in_row) * 16, take ? k + c * 16 : none, take);
-              copy_16(to + L::GB + piece<L::CPR, true>(row, in_row) * 16, take ? v + c * 16 : none, take);
+              copy_16(to + piece<L::CPR, F8, false>(row, in_row) * 16, take ? k + c * 16 : none, take);
+              copy_16(to + L::GB + piece<L::CPR, F8, true>(row, in_row) * 16, take ? v + c * 16 : none, take);
             }
           }
         }
@@ -810,9 +834,11 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
             join_l[warp][row] = r.l[n][h];
           }
 #pragma unroll
-          for (int y = 0; y < HD / 16; ++y)
-            *reinterpret_cast<float2*>(o_at + (warp * kRows + row) * HD + column<HD, F8>(2 * y, g)) =
-                make_float2(r.o[n][y][h] * unit_o, r.o[n][y][2 + h] * unit_o);
+          for (int y = 0; y < HD / 16; ++y) {
+            float* at = o_at + (warp * kRows + row) * HD;
+            at[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
+            at[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
+          }
         }
       __syncthreads();
       const int n_rows = done.s.n * a.group;
@@ -842,24 +868,43 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
       }
     } else {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int n = 0; n < NB; ++n) {
+        const int rows = done.s.n * a.group - done.mt * kRows;  // of the tile
+        if (complete) {
+          float by[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = warp_rows + 8 * n + 2 * j + h, at = done.mt * kRows + row;
-          if (at >= done.s.n * a.group) continue;
-          const float by = complete ? (r.l[n][h] == 0.f ? 0.f : unit_o / r.l[n][h]) : unit_o;
-          const int t = a.by_group(at), hd = at - t * a.group;
+          for (int h = 0; h < 2; ++h) by[h] = r.l[n][h] == 0.f ? 0.f : unit_o / r.l[n][h];
+          // transposed: columns 2 j and 2 j + 1 of a group of eight, or of pairs of them, for row g
+          const int row = warp_rows + 8 * n + g, at = done.mt * kRows + row, t = a.by_group(at), hd = at - t * a.group;
           bf16* out = a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD;
-          float* part = a.part + ((size_t)slot * kRows + row) * HD;
-          if (!complete && g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h], r.l[n][h]);
 #pragma unroll
           for (int y = 0; y < HD / 16; ++y) {
-            const int col = column<HD, F8>(2 * y, g);
-            const float u = r.o[n][y][h] * by, v = r.o[n][y][2 + h] * by;
-            if (complete) *reinterpret_cast<uint32_t*>(out + col) = pack<false>(u, v);
-            else *reinterpret_cast<float2*>(part + col) = make_float2(u, v);
+            const uint32_t u = transposed(pack<false>(r.o[n][y][0] * by[0], r.o[n][y][1] * by[1]));
+            const uint32_t v = transposed(pack<false>(r.o[n][y][2] * by[0], r.o[n][y][3] * by[1]));
+            if (row >= rows) continue;
+            if (F8) {  // element 2 y and element 2 y + 1, neighbours, of threads 2 j and 2 j + 1
+              *reinterpret_cast<uint32_t*>(out + column<HD, F8>(2 * y, 2 * j)) = __byte_perm(u, v, 0x5410);
+              *reinterpret_cast<uint32_t*>(out + column<HD, F8>(2 * y, 2 * j + 1)) = __byte_perm(u, v, 0x7632);
+            } else {
+              *reinterpret_cast<uint32_t*>(out + 16 * y + 2 * j) = u;
+              *reinterpret_cast<uint32_t*>(out + 16 * y + 8 + 2 * j) = v;
+            }
+          }
+          continue;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = warp_rows + 8 * n + 2 * j + h;
+          if (row >= rows) continue;
+          float* part = a.part + ((size_t)slot * kRows + row) * HD;
+          if (g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h], r.l[n][h]);
+#pragma unroll
+          for (int y = 0; y < HD / 16; ++y) {
+            part[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
+            part[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
           }
         }
+      }
     }
     if (!complete && begins && tid == 0) {
       // parts: this CTA's and one of each of the next ones until the item ends
@@ -951,21 +996,49 @@ __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int 
       make_uint2(pack<false>(o.x * by, o.y * by), pack<false>(o.z * by, o.w * by));
 }
 
-// One row of one shared item a time.  Most CTAs of the first kernel begin none: 32 of them are looked at together.
+// The same by a warp, for a few parts.
+template <int HD, int kRows>
+__device__ __forceinline__ void join_row_by_warp(const Attn& a, int cta, int4 item, int row) {
+  const Span s = span_of(a.batch, item.x, INT32_MAX, INT32_MAX, a.status);
+  const int at = item.y * kRows + row, parts = item.w, lane = threadIdx.x & 31;
+  if (at >= s.n * a.group) return;
+  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row; };
+  float2 st = lane < parts ? a.stats[slot(lane)] : make_float2(-INFINITY, 0.f);
+  const float m = warp_max(st.x), f = exp2_fast(st.x - (m == -INFINITY ? 0.f : m)), l = warp_sum(st.y * f), by = l == 0.f ? 0.f : 1.f / l;
+  const int t = a.by_group(at), hd = at - t * a.group;
+  bf16* out = a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(item.z * a.group + hd) * HD;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float fi = __shfl_sync(0xffffffffu, f, i) * by;
+    if (lane * 4 >= HD) continue;
+    const float4 v = *reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4);
+    o.x = fmaf(v.x, fi, o.x); o.y = fmaf(v.y, fi, o.y); o.z = fmaf(v.z, fi, o.z); o.w = fmaf(v.w, fi, o.w);
+  }
+  if (lane * 4 < HD) *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack<false>(o.x, o.y), pack<false>(o.z, o.w));
+}
+
+// Rows of shared items, task t: row t % rows of the item that begins in CTA t / rows.  Most CTAs of the first kernel begin none: 32 tasks are
+// looked at together.  Items of up to kFew parts take a warp a row, eight rows from every eighth task, others a block.  The
+// grid's size is odd where a block has several tasks, so that those are spread evenly.
 template <int HD, int kRows>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int ctas, int rows) {
+  constexpr int kFew = 6, kWarps = kJoinThreads / 32;
   pdl_trigger();
   pdl_wait();
-  // this block's tasks: blockIdx.x, + gridDim.x, ...; task t is row t % rows of CTA t / rows
-  const int lane = threadIdx.x & 31, tasks = ctas * rows;
+  const int lane = threadIdx.x & 31, tasks = ctas * rows;  // this block's: blockIdx.x, + gridDim.x, ...
   for (int t0 = blockIdx.x; t0 < tasks; t0 += 32 * gridDim.x) {
-    const int mine = t0 + lane * (int)gridDim.x;
-    const int4 item = mine < tasks ? a.head[mine / rows] : make_int4(-1, 0, 0, 0);
-    for (uint32_t left = __ballot_sync(0xffffffffu, item.x >= 0); left; left &= left - 1) {
-      const int from = __ffs(left) - 1, t = t0 + from * (int)gridDim.x;
+    const int mine = t0 + lane * (int)gridDim.x, my_cta = mine / rows, my_row = mine - my_cta * rows;
+    const int4 item = mine < tasks ? a.head[my_cta] : make_int4(-1, 0, 0, 0);
+    for (uint32_t left = __ballot_sync(0xffffffffu, item.x >= 0 && (item.w > kFew || my_row % kWarps == 0)); left; left &= left - 1) {
+      const int from = __ffs(left) - 1, cta = __shfl_sync(0xffffffffu, my_cta, from), row = __shfl_sync(0xffffffffu, my_row, from);
       const int4 one = make_int4(__shfl_sync(0xffffffffu, item.x, from), __shfl_sync(0xffffffffu, item.y, from),
                                  __shfl_sync(0xffffffffu, item.z, from), __shfl_sync(0xffffffffu, item.w, from));
-      join_row<HD, kRows>(a, t / rows, one, t % rows);
+      if (one.w <= kFew) {
+        if (row + (int)(threadIdx.x >> 5) < rows) join_row_by_warp<HD, kRows>(a, cta, one, row + (threadIdx.x >> 5));
+        continue;
+      }
+      join_row<HD, kRows>(a, cta, one, row);
       __syncthreads();
     }
   }
@@ -996,7 +1069,7 @@ cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
   cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(F::kThreads), a.stages * F::kStage, s, a);
   if (e != cudaSuccess || !may_share) return e;
   const int rows = (int)min((long long)kRows, (long long)a.max_new * a.group);
-  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, 4ll * sms)), dim3(kJoinThreads), 0, s, a, ctas, rows);
+  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, 4ll * sms - 1)), dim3(kJoinThreads), 0, s, a, ctas, rows);
 }
 
 // Rows of one KV head at most: which form.
