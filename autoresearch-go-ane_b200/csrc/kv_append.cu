@@ -31,54 +31,65 @@ struct Append {
   int ld_qkv, ld_q, heads, n_positions;
   int rows_blocks;  // blocks that rotate rows; the others are 8-bit pages
   int units;        // bound of the pages that are touched
+  int capacity;     // tokens of a sequence
+  int q_vec, kv_vec;  // groups of eight elements of a row's queries, and keys or values, that the former take
+  Div by_row, by_head, by_page;  // by those groups of a row, by groups of a head, by tokens of a page
   int* status;
 };
 
-// The last sequence whose first row is not behind `row` (a block's threads compare one sequence each, which is one round trip to
-// memory where a binary search takes one for each halving); n_seq if all rows of sequences lie before it.
-template <int T, class Less>
-__device__ __forceinline__ int count_before(int n, int lane, Less before) {
-  int c = 0;
-  for (int i = lane; i < n; i += T) c += before(i) ? 1 : 0;
+// The first sequence whose end, as end(i) gives it for start[i + 1], lies behind `at`, and what the batch says of it: all of a team's T threads
+// look at other sequences, so that this takes one round trip to memory.  n_seq if there is none.
+struct Found {
+  int b, row, end, pos;
+};
+template <int T, class End>
+__device__ __forceinline__ Found find(const Batch& a, int at, int lane, End end) {
+  Found f = {a.n_seq, 0, 0, 0};
+  bool mine = false;
+  for (int i = lane; i < a.n_seq && !mine; i += T) {
+    const int from = a.start[i], to = a.start[i + 1], pos = a.pos[i];
+    mine = end(to, i + 1) > at && (i == 0 || end(from, i) <= at);
+    if (mine) f = {i, from, to, pos};
+  }
   if constexpr (T == 32) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-    return c;
+    const uint32_t who = __ballot_sync(0xffffffffu, mine);
+    const int from = who ? __ffs(who) - 1 : 0;
+    return {__shfl_sync(0xffffffffu, f.b, from), __shfl_sync(0xffffffffu, f.row, from), __shfl_sync(0xffffffffu, f.end, from),
+            __shfl_sync(0xffffffffu, f.pos, from)};
   } else {
-    __shared__ int part[T / 32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-    if ((lane & 31) == 0) part[lane >> 5] = c;
+    __shared__ Found found;
+    if (lane == 0) found = {a.n_seq, 0, 0, 0};
     __syncthreads();
-    c = 0;
-#pragma unroll
-    for (int i = 0; i < T / 32; ++i) c += part[i];
-    return c;
+    if (mine) found = f;
+    __syncthreads();
+    return found;
   }
 }
 
-// Eight elements of a row, rotated where cos / sin are given.  Products and sums are rounded one by one.
+// Eight elements of a row, rotated by their position if c is given.  Products and sums are rounded one by one.
 struct Eight {
   float x[8];
 };
-__device__ __forceinline__ Eight load_eight(const bf16* p, const float* c, const float* s) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw {
+  uint4 x;
+  float4 c, s;
+};
+__device__ __forceinline__ Raw fetch_eight(const bf16* p, const float* c, const float* s) {
+  Raw r;
+  r.x = *reinterpret_cast<const uint4*>(p);
+  r.c = c ? *reinterpret_cast<const float4*>(c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  r.s = c ? *reinterpret_cast<const float4*>(s) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return r;
+}
+__device__ __forceinline__ Eight turned(const Raw& r, bool turn) {
+  const uint32_t w[4] = {r.x.x, r.x.y, r.x.z, r.x.w};
+  const float c[4] = {r.c.x, r.c.y, r.c.z, r.c.w}, s[4] = {r.s.x, r.s.y, r.s.z, r.s.w};
   Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    e.x[2 * i] = __uint_as_float(w[i] << 16);
-    e.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-  if (c) {
-    const float4 c4 = *reinterpret_cast<const float4*>(c), s4 = *reinterpret_cast<const float4*>(s);
-    const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = e.x[2 * i], b = e.x[2 * i + 1];
-      e.x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
-      e.x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cc[i]), __fmul_rn(a, ss[i]));
-    }
+    const float a = __uint_as_float(w[i] << 16), b = __uint_as_float(w[i] & 0xffff0000u);
+    e.x[2 * i] = turn ? __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i])) : a;
+    e.x[2 * i + 1] = turn ? __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i])) : b;
   }
   return e;
 }
@@ -93,49 +104,61 @@ __device__ __forceinline__ void store_eight(bf16* p, const Eight& e) {
 }
 
 // kEach * kThreads groups of eight elements of the tokens' rows, in the order of memory: the queries of all caches, keys and values too of a
-// bf16 one.
+// bf16 one.  All of a thread's loads are on their way before the first is used.
 __device__ __forceinline__ void append_rows(const Append& a, int block) {
-  const int tid = threadIdx.x;
-  const int hd = a.kv.head_dim, half = hd >> 1, page = a.kv.page_size;
-  const int capacity = (int)min((long long)a.kv.table_pitch * page, (long long)INT32_MAX);
-  const int q_vec = a.q ? a.heads * hd / 8 : 0, kv_vec = a.kv.e4m3 ? 0 : a.kv.kv_heads * hd / 8, vec = q_vec + 2 * kv_vec;
-  const long long begin = (long long)block * (kEach * kThreads);
-  const int first = (int)(begin / vec), v0 = (int)(begin - (long long)first * vec);
+  const int tid = threadIdx.x, hd = a.kv.head_dim, half = hd >> 1, page = a.kv.page_size;
+  const int vec = a.q_vec + 2 * a.kv_vec, begin = block * (kEach * kThreads), first = a.by_row(begin);
   // the sequence of the block's first row; the next ones are found from there
-  int b = count_before<kThreads>(a.batch.n_seq, tid, [&](int i) { return a.batch.start[i + 1] <= first; });
-  Span s = {0, 0, 0};
-  int known = -1;
+  const Found f = find<kThreads>(a.batch, first, tid, [](int to, int) { return to; });
+  int b = f.b, end = f.end;
+  Span s = span_of(f.row, f.end, f.pos, a.batch, a.capacity, INT32_MAX, a.status);
+  Raw raw[kEach];
+  bf16* to[kEach];
+  int number[kEach];  // of the page
+  uint32_t turn = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int u = v0 + tid + i * kThreads, row = first + u / vec, v = u % vec;
-    if (row >= a.batch.n_tokens) break;
-    while (b < a.batch.n_seq && a.batch.start[b + 1] <= row) ++b;
-    if (b == a.batch.n_seq) break;
-    if (b != known) s = span_of(a.batch, known = b, capacity, INT32_MAX, a.status);
-    if (s.n == 0 || row < s.row) continue;
+    const int u = begin + tid + i * kThreads, row = a.by_row(u), v = u - row * vec;
+    to[i] = nullptr;
+    number[i] = 0;
+    if (row >= a.batch.n_tokens) continue;
+    while (b < a.batch.n_seq && end <= row)
+      if (++b < a.batch.n_seq) {
+        end = a.batch.start[b + 1];
+        s = span_of(a.batch, b, a.capacity, INT32_MAX, a.status);
+      }
+    if (b == a.batch.n_seq || s.n == 0 || row < s.row) continue;
     const int pos = s.pos + row - s.row;
-    const int part = v < q_vec ? 0 : v < q_vec + kv_vec ? 1 : 2;
-    const int col = (part == 0 ? v : v - q_vec - (part - 1) * kv_vec) * 8;  // within q, k or v
-    const bool turn = part < 2 && a.cosb;
-    if (turn && pos >= a.n_positions) {
-      atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
-      continue;
+    const int part = v < a.q_vec ? 0 : v < a.q_vec + a.kv_vec ? 1 : 2;
+    const int in_part = part == 0 ? v : v - a.q_vec - (part - 1) * a.kv_vec;  // within q, k or v
+    const int head = a.by_head(in_part), in_head = in_part * 8 - head * hd;
+    if (part < 2 && a.cosb) {
+      if (pos >= a.n_positions) {
+        atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
+        continue;
+      }
+      turn |= 1u << i;
     }
-    const int in_col = col + (part == 0 ? 0 : (a.heads + (part - 1) * a.kv.kv_heads) * hd);
-    const int head = col / hd, in_head = col - head * hd;
     const size_t at = (size_t)pos * half + (in_head >> 1);
-    const Eight e = load_eight(a.qkv + (size_t)row * a.ld_qkv + in_col, turn ? a.cosb + at : nullptr, turn ? a.sinb + at : nullptr);
+    const bf16* from = a.qkv + (size_t)row * a.ld_qkv + (part == 0 ? 0 : (a.heads + (part - 1) * a.kv.kv_heads) * hd) + in_part * 8;
+    const bool turns = turn >> i & 1;
+    raw[i] = fetch_eight(from, turns ? a.cosb + at : nullptr, turns ? a.sinb + at : nullptr);
     if (part == 0) {
-      store_eight(a.q + (size_t)row * a.ld_q + col, e);
-      continue;
+      to[i] = a.q + (size_t)row * a.ld_q + in_part * 8;
+    } else {
+      const int slot = a.by_page(pos);
+      number[i] = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
+      to[i] = reinterpret_cast<bf16*>(part == 1 ? a.kv.k : a.kv.v) + ((size_t)head * page + pos - slot * page) * hd + in_head;
     }
-    const int slot = pos / page, p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
-    if (p < 0 || p >= a.kv.n_pages) {
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (!to[i]) continue;
+    if ((unsigned)number[i] >= (unsigned)a.kv.n_pages) {
       atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
       continue;
     }
-    bf16* cache = reinterpret_cast<bf16*>(part == 1 ? a.kv.k : a.kv.v);
-    store_eight(cache + p * a.kv.page_stride + ((size_t)head * page + pos - slot * page) * hd + in_head, e);
+    store_eight(to[i] + number[i] * a.kv.page_stride, turned(raw[i], turn >> i & 1));
   }
 }
 
@@ -162,47 +185,64 @@ __device__ __forceinline__ uint2 to_e4m3(const Eight& e, float scale, bool power
 }
 
 // One page and head of 8-bit keys or values by a team of T threads: the largest new value gives the scale, then the new rows
-// are rounded, and the rows that the page held before if the scale has grown.  The page's rows are read twice: the
-// second time they are in L1 or L2.
+// are rounded, and the rows that the page held before if the scale has grown.  A thread keeps its first kKeep groups of eight in registers;
+// others are read again, from L1 or L2.
 //
 // Unit u is a page that some sequence touches, found without a list: with U(b) = start[b] / page_size + 2 b sequence b has the
 // units U(b) .. U(b + 1) - 1, at least as many as the pages its tokens can touch.
 template <int T>
 __device__ __forceinline__ void append_page(const Append& a, int unit, int head, bool values, int lane) {
+  constexpr int kKeep = T == 32 ? 2 : 4;
   const int hd = a.kv.head_dim, half = hd >> 1, page = a.kv.page_size;
-  const int capacity = (int)min((long long)a.kv.table_pitch * page, (long long)INT32_MAX);
-  const int b = count_before<T>(a.batch.n_seq, lane, [&](int i) { return a.batch.start[i + 1] / page + 2 * (i + 1) <= unit; });
+  const Found f = find<T>(a.batch, unit, lane, [&](int to, int i) { return a.by_page(max(to, 0)) + 2 * i; });
+  const int b = f.b;
   if (b >= a.batch.n_seq) return;
-  const Span s = span_of(a.batch, b, capacity, INT32_MAX, a.status);
-  const int ahead = unit - (a.batch.start[b] / page + 2 * b), slot = s.pos / page + ahead;
-  if (s.n == 0 || ahead < 0 || slot > (s.pos + s.n - 1) / page) return;
+  const Span s = span_of(f.row, f.end, f.pos, a.batch, a.capacity, INT32_MAX, a.status);
+  if (s.n == 0) return;
+  const int ahead = unit - (a.by_page(s.row) + 2 * b), slot = a.by_page(s.pos) + ahead;
+  if (ahead < 0 || slot > a.by_page(s.pos + s.n - 1)) return;
   const int p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
-  if (p < 0 || p >= a.kv.n_pages || (!values && a.cosb && s.pos + s.n > a.n_positions)) {
+  const bool turn = !values && a.cosb;
+  if (turn && s.pos + s.n > a.n_positions) {
     if (lane == 0) atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
     return;
   }
   const int page0 = slot * page;
   const int lo = max(s.pos, page0) - page0, hi = min(s.pos + s.n, page0 + page) - page0;  // new rows of the page
   const bf16* in = a.qkv + (size_t)(s.row + page0 + lo - s.pos) * a.ld_qkv + (a.heads + (values ? a.kv.kv_heads : 0) + head) * hd;
-  const bool turn = !values && a.cosb;
   const float* c = turn ? a.cosb + (size_t)(page0 + lo) * half : nullptr;
   const float* n = turn ? a.sinb + (size_t)(page0 + lo) * half : nullptr;
   const int per_row = hd / 8, vecs = (hi - lo) * per_row;
-  auto load = [&](int i) {
-    const int r = i / per_row, v = i - r * per_row;
+  auto fetch = [&](int i) {
+    const int r = a.by_head(i), v = i - r * per_row;
     const size_t at = (size_t)r * half + v * 4;
-    return load_eight(in + (size_t)r * a.ld_qkv + v * 8, turn ? c + at : nullptr, turn ? n + at : nullptr);
+    return fetch_eight(in + (size_t)r * a.ld_qkv + v * 8, turn ? c + at : nullptr, turn ? n + at : nullptr);
   };
+  // the rows are on their way while the page's number arrives
+  Raw raw[kKeep];
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (lane + k * T < vecs) raw[k] = fetch(lane + k * T);
+  if (p < 0 || p >= a.kv.n_pages) {
+    if (lane == 0) atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
+    return;
+  }
+  float* scale_at = (values ? a.kv.v_scale : a.kv.k_scale) + (size_t)p * a.kv.kv_heads + head;
+  const float old = lo > 0 ? *scale_at : 0.f;
   float top = 0.f;
-#pragma unroll 4
-  for (int i = lane; i < vecs; i += T) {
-    const Eight e = load(i);
+  auto look_at = [&](const Eight& e) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float x = fabsf(e.x[j]);
       if (x <= 3.402823466e38f) top = fmaxf(top, x);  // not what is infinite or NaN
     }
-  }
+  };
+  Eight kept[kKeep];
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (lane + k * T < vecs) look_at(kept[k] = turned(raw[k], turn));
+#pragma unroll 4
+  for (int i = lane + kKeep * T; i < vecs; i += T) look_at(turned(fetch(i), turn));
   top = warp_max(top);
   if constexpr (T > 32) {
     __shared__ float tops[T / 32];
@@ -211,8 +251,6 @@ __device__ __forceinline__ void append_page(const Append& a, int unit, int head,
 #pragma unroll
     for (int i = 0; i < T / 32; ++i) top = fmaxf(top, tops[i]);
   }
-  float* scale_at = (values ? a.kv.v_scale : a.kv.k_scale) + (size_t)p * a.kv.kv_heads + head;
-  const float old = lo > 0 ? *scale_at : 0.f;
   const float scale = fmaxf(old, __uint_as_float((uint32_t)(scale_exponent(top) + 127) << 23));
   unsigned char* out = reinterpret_cast<unsigned char*>(values ? a.kv.v : a.kv.k) + p * a.kv.page_stride + (size_t)head * page * hd;
   if (T > 32) __syncthreads();
@@ -220,9 +258,13 @@ __device__ __forceinline__ void append_page(const Append& a, int unit, int head,
   if (lane == 0) *scale_at = scale;  // all have read it
   const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale < 1.7014118e38f;
   const float inverse = power ? __uint_as_float((254u << 23) - __float_as_uint(scale)) : 0.f;
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (lane + k * T < vecs)
+      *reinterpret_cast<uint2*>(out + (size_t)lo * hd + (size_t)(lane + k * T) * 8) = to_e4m3(kept[k], scale, power, inverse);
 #pragma unroll 4
-  for (int i = lane; i < vecs; i += T)
-    *reinterpret_cast<uint2*>(out + (size_t)lo * hd + (size_t)i * 8) = to_e4m3(load(i), scale, power, inverse);
+  for (int i = lane + kKeep * T; i < vecs; i += T)
+    *reinterpret_cast<uint2*>(out + (size_t)lo * hd + (size_t)i * 8) = to_e4m3(turned(fetch(i), turn), scale, power, inverse);
   if (lo > 0 && old != scale) {
     const float ratio = __fdiv_rn(old, scale);
     for (int i = lane; i < lo * per_row; i += T) {
@@ -261,9 +303,17 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const Append a) {
 cudaError_t kv_append(const PagedKv& kv, const Batch& batch, int heads, const bf16* qkv, int ld_qkv, bf16* q, int ld_q,
                       const float* cosb, const float* sinb, int n_positions, int* status, cudaStream_t s) {
   if (batch.n_seq == 0 || batch.n_tokens == 0) return cudaSuccess;
-  Append a = {kv, batch, qkv, q, cosb, sinb, ld_qkv, ld_q, heads, n_positions, 0, 0, status};
-  const long long vec = (long long)batch.n_tokens * ((q ? heads : 0) + (kv.e4m3 ? 0 : 2 * kv.kv_heads)) * kv.head_dim / 8;
-  if ((vec + kEach * kThreads - 1) / (kEach * kThreads) > INT32_MAX) return cudaErrorInvalidValue;
+  Append a = {kv, batch, qkv, q, cosb, sinb, ld_qkv, ld_q, heads, n_positions};
+  a.status = status;
+  a.capacity = (int)min((long long)kv.table_pitch * kv.page_size, (long long)INT32_MAX);
+  a.q_vec = q ? heads * kv.head_dim / 8 : 0;
+  a.kv_vec = kv.e4m3 ? 0 : kv.kv_heads * kv.head_dim / 8;
+  const int row_vec = a.q_vec + 2 * a.kv_vec;
+  a.by_row = Div(row_vec ? row_vec : 1);
+  a.by_head = Div(kv.head_dim / 8);
+  a.by_page = Div(kv.page_size);
+  const long long vec = (long long)batch.n_tokens * row_vec;
+  if (vec > INT32_MAX - kEach * kThreads) return cudaErrorInvalidValue;
   a.rows_blocks = (int)((vec + kEach * kThreads - 1) / (kEach * kThreads));
   long long tasks = 0;
   if (kv.e4m3) {

@@ -30,17 +30,6 @@ constexpr float kSlack = 8.f;
 constexpr float kPScale = 128.f;  // of f16 probabilities, 2^15 at most then: those down to 2^-21 of the maximum's stay normal
 constexpr float kLowest = 1.17549435e-38f;
 
-// Quotients by a number known at launch, in five instructions: floor(2^32 / d) gives them or one less.
-struct Div {
-  uint32_t d, m;
-  Div() = default;
-  explicit Div(int by) : d(by), m(by == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / by)) {}
-  __device__ __forceinline__ int operator()(int n) const {
-    const uint32_t q = __umulhi((uint32_t)n, m);
-    return (int)(q + ((uint32_t)n - q * d >= d ? 1u : 0u));
-  }
-};
-
 struct Attn {
   PagedKv kv;
   Batch batch;

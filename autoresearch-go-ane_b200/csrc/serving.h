@@ -37,18 +37,31 @@ size_t kv_attention_workspace(int sms, int head_dim);
 cudaError_t logit_rules(const ane_logit_rules_args& a, int* status, cudaStream_t s);
 
 #ifdef __CUDACC__
+// Quotients by a number known at launch, in five instructions: floor(2^32 / d) gives them or one less.
+struct Div {
+  uint32_t d, m;
+  Div() = default;
+  explicit Div(int by) : d(by), m(by == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / by)) {}
+  __device__ __forceinline__ int operator()(int n) const {
+    const uint32_t q = __umulhi((uint32_t)n, m);
+    return (int)(q + ((uint32_t)n - q * d >= d ? 1u : 0u));
+  }
+};
+
 // New rows and place of sequence b; none (and the status word) where its entries make no sense.
 struct Span {
   int row, n, pos;
 };
-__device__ __forceinline__ Span span_of(const Batch& a, int b, int capacity, int most, int* status) {
-  const int row = a.start[b], end = a.start[b + 1], pos = a.pos[b];
+__device__ __forceinline__ Span span_of(int row, int end, int pos, const Batch& a, int capacity, int most, int* status) {
   if (row == end) return {row, 0, pos};
   if (row < 0 || end < row || end > a.n_tokens || end - row > most || pos < 0 || end - row > capacity - pos) {
     atomicCAS(status, DEV_OK, DEV_BAD_INDEX);
     return {row, 0, pos};
   }
   return {row, end - row, pos};
+}
+__device__ __forceinline__ Span span_of(const Batch& a, int b, int capacity, int most, int* status) {
+  return span_of(a.start[b], a.start[b + 1], a.pos[b], a, capacity, most, status);
 }
 #endif
 

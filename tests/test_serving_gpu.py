@@ -496,7 +496,7 @@ def test_rules_match_their_definition(dtype, rows, vocab):
 
 @pytest.mark.parametrize("kw", [
     dict(history=0), dict(history=0, masks=3), dict(history=0, masks=3, by_row=False), dict(history=0, biases=9), dict(history=1),
-    dict(history=5000), dict(history=40000, biases=9), dict(history=200, penalties="r"), dict(history=200, penalties="p"), dict(history=200, penalties="f"),
+    dict(history=5000), dict(history=6000, biases=700), dict(history=12000, biases=700), dict(history=40000, biases=9), dict(history=200, penalties="r"), dict(history=200, penalties="p"), dict(history=200, penalties="f"),
     dict(history=200, penalties=""), dict(history=200, n_prompt=False), dict(history=200, biases=9, masks=2, in_place=True),
     dict(history=200, biases=9, masks=2, in_place=True, pad=3),
 ])
