@@ -438,7 +438,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 mat
 
 // KG * 16 keys at positions key0.. against the warp's rows; group i of them lies at ring + i * 2 * GB.  `checked`: some row does not
 // see some key.
-template <int HD, bool F8, int NB, int KG>
+template <int HD, bool F8, int NB, int KG, bool kRest>
 __device__ __forceinline__ void take_keys(const char* ring, const float2* scales, int key0, bool checked, int window, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
   constexpr int kChains = NB == 1 ? 2 : 1;
@@ -522,7 +522,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
 #pragma unroll
     for (int k = 0; k < KG; ++k) into[k] = scale[k].y * r.v_inv;
   }
-  uint32_t p[KG][NB][2];
+  uint32_t p[KG][NB][2], rest[kRest ? KG : 1][NB][2];
   bool above = false;
   float mult[KG][NB][2];
 #pragma unroll
@@ -575,7 +575,8 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
       }
       r.l[n][h] += sum;  // the thread's own keys; joined at the end
     }
-    // probabilities in 16 bits: their rounding is half a step of the output's own type or less
+    // Probabilities in 16 bits.  f16 is finer than the output's type.  bf16 is as coarse, and errors of both add up to 1.4 times the output's own;
+    // where products cost nothing, for few rows, what rounding has left of it is added.
 #pragma unroll
     for (int k = 0; k < KG; ++k) {
       if (F8) {
@@ -584,6 +585,13 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
       }
       p[k][n][0] = transposed(pack<F8>(s[k][n][0], s[k][n][1]));
       p[k][n][1] = transposed(pack<F8>(s[k][n][2], s[k][n][3]));
+      if constexpr (kRest) {
+        float left[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) left[i] = s[k][n][i] - __bfloat162float(__float2bfloat16_rn(s[k][n][i]));
+        rest[k][n][0] = transposed(pack<F8>(left[0], left[1]));
+        rest[k][n][1] = transposed(pack<F8>(left[2], left[3]));
+      }
     }
   }
   if (checked) {
@@ -634,7 +642,10 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
         uint32_t v[4];
         load_matrices<true>(at + piece<L::CPR, F8, true>((lane & 7) + (lane >> 4) * 8, 2 * y + (lane >> 3 & 1)) * 16, v);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) mma<false>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+        for (int n = 0; n < NB; ++n) {
+          mma<false>(r.o[n][y], v, p[k][n][0], p[k][n][1]);
+          if constexpr (kRest) mma<false>(r.o[n][y], v, rest[k][n][0], rest[k][n][1]);
+        }
       }
     }
 #pragma unroll
@@ -787,7 +798,7 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
         const int key0 = key_tile + w * kGroup;
         if (!any_row || key0 > p_last || (a.window && key0 + KG * kGroup - 1 <= p_first - a.window)) continue;
         const bool checked = key0 + KG * kGroup - 1 > p_first || (a.window && key0 <= p_last - a.window);
-        take_keys<HD, F8, NB, KG>(at + w * 2 * L::GB, &scales[from_stage][w], key0, checked, a.window, r);
+        take_keys<HD, F8, NB, KG, kSplit && !F8>(at + w * 2 * L::GB, &scales[from_stage][w], key0, checked, a.window, r);
       }
       if (++from_stage == a.stages) from_stage = 0;
     }
