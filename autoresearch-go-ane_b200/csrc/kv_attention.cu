@@ -62,7 +62,7 @@ struct Form {
   using L = Layout<HD, F8>;
   static constexpr int kGroups = kSplit ? (L::RB <= 64 && NB == 1 ? 2 : 1) : 2;
   // groups of 16 keys of a tile that a warp fetches; the ring has to hold the outputs of kSplit's warps
-  static constexpr int kLoads = kSplit || L::RB <= 128 ? kGroups : 1;
+  static constexpr int kLoads = kSplit ? (kGroups * 3 * L::ES < NB ? 2 : kGroups) : L::RB <= 128 ? kGroups : 1;
   static constexpr int kThreads = 32 * kWarps, kTile = kGroup * kWarps * kLoads;
   static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
   static constexpr int kStage = kWarps * kLoads * 2 * L::GB;
@@ -1078,6 +1078,8 @@ cudaError_t run_rows(const Attn& a, int sms, void* workspace, cudaStream_t s) {
   const long long rows = (long long)a.max_new * a.group;
   if (rows <= 8) return run<Form<HD, F8, 1, true>>(a, sms, workspace, s);
   if (rows <= 16) return run<Form<HD, F8, 2, true>>(a, sms, workspace, s);
+  if constexpr (HD <= 64)
+    if (rows <= 32) return run<Form<HD, F8, 4, true>>(a, sms, workspace, s);
   return run<Form<HD, F8, HD <= 64 ? 4 : 2, false>>(a, sms, workspace, s);
 }
 template <int HD>
