@@ -102,6 +102,15 @@ class LogitRulesArgs(ctypes.Structure):
     ]
 
 
+class GenerateArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", c_uint32), ("n_seq", c_uint32), ("prompts", POINTER(c_uint16)), ("prompt_len", POINTER(c_uint32)), ("n_new", c_uint32),
+        ("kv_dtype", c_int32), ("temperature", c_float), ("repetition", c_float), ("presence", c_float), ("frequency", c_float),
+        ("uniforms", POINTER(c_double)), ("allowed", POINTER(c_uint32)), ("bias_token", POINTER(c_int32)), ("bias", POINTER(c_float)),
+        ("n_bias", c_uint32), ("pad_", c_uint32), ("out", POINTER(c_uint16)),
+    ]
+
+
 # Every symbol include/ane_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "ane_device_count": (c_int32, []),
@@ -144,6 +153,7 @@ SIGNATURES = {
     "ane_decode_greedy": (c_int32, [c_void_p, POINTER(c_uint16), c_uint32, c_uint32, c_uint32, POINTER(c_uint16)]),
     "ane_decode_sample": (c_int32, [c_void_p, POINTER(c_uint16), c_uint32, c_uint32, c_uint32, c_float, POINTER(c_double),
                                     POINTER(c_uint16)]),
+    "ane_generate": (c_int32, [c_void_p, POINTER(GenerateArgs)]),
     "ane_set_lr": (c_int32, [c_void_p, c_float]),
     "ane_get_lr": (c_float, [c_void_p]),
     "ane_get_state": (c_int32, [c_void_p, POINTER(State)]),

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import weakref
-from ctypes import POINTER, byref, c_double, c_float, c_uint8, c_uint16, c_uint64, c_void_p
+from ctypes import POINTER, byref, c_double, c_float, c_int32, c_uint8, c_uint16, c_uint32, c_uint64, c_void_p
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -258,6 +258,43 @@ class Engine:
         out = np.empty((n_seq, n_new), dtype=np.uint16)
         self._check(lib.ane_decode_sample(self._h, _u16p(prompts), n_seq, plen, n_new, temperature,
                                           uniforms.ctypes.data_as(POINTER(c_double)), _u16p(out)))
+        return out
+
+    def generate(self, prompts, n_new: int, kv: str = "bf16", temperature: float = 0.0, uniforms: np.ndarray | None = None,
+                 repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias: dict | None = None,
+                 allowed: np.ndarray | None = None) -> np.ndarray:
+        """Generation over a paged KV cache of type `kv` ("bf16" or "e4m3"): prompts are token arrays of any lengths, the result is
+        [len(prompts), n_new].  `bias` maps tokens to what is added to their logits, `allowed` holds a truth value for each token of the
+        vocabulary; `uniforms` [n_new, len(prompts)] as for decode_sample."""
+        self._alive("generate")
+        if kv not in ("bf16", "e4m3"):
+            raise EngineError(-1, f"storiesane generate: kv={kv!r} want 'bf16' or 'e4m3'")
+        rows = [np.ascontiguousarray(p, dtype=np.uint16).ravel() for p in prompts]
+        flat = np.concatenate(rows) if rows else np.zeros(0, np.uint16)
+        lens = np.array([r.size for r in rows], dtype=np.uint32)
+        out = np.empty((len(rows), n_new), dtype=np.uint16)
+        a = _ffi.GenerateArgs(struct_size=ctypes.sizeof(_ffi.GenerateArgs), n_seq=len(rows), prompts=_u16p(flat),
+                              prompt_len=lens.ctypes.data_as(POINTER(c_uint32)), n_new=n_new,
+                              kv_dtype=_ffi.KV_E4M3 if kv == "e4m3" else _ffi.KV_BF16, temperature=temperature, repetition=repetition,
+                              presence=presence, frequency=frequency, out=_u16p(out))
+        if uniforms is not None:
+            uniforms = np.ascontiguousarray(uniforms, dtype=np.float64)
+            if uniforms.shape != (n_new, len(rows)):
+                raise EngineError(-1, f"storiesane generate: uniforms shape={uniforms.shape} want={(n_new, len(rows))}")
+            a.uniforms = uniforms.ctypes.data_as(POINTER(c_double))
+        if allowed is not None:
+            allowed = np.asarray(allowed, dtype=bool).ravel()
+            if allowed.size != self.vocab:
+                raise EngineError(-1, f"storiesane generate: allowed len={allowed.size} want={self.vocab}")
+            words = np.zeros((self.vocab + 31) // 32 * 32, dtype=bool)
+            words[:self.vocab] = allowed
+            words = np.ascontiguousarray(np.packbits(words, bitorder="little")).view(np.uint32)
+            a.allowed = words.ctypes.data_as(POINTER(c_uint32))
+        if bias:
+            tokens, values = np.array(list(bias.keys()), dtype=np.int32), np.array(list(bias.values()), dtype=np.float32)
+            a.bias_token, a.bias = tokens.ctypes.data_as(POINTER(c_int32)), values.ctypes.data_as(POINTER(c_float))
+            a.n_bias = tokens.size
+        self._check(lib.ane_generate(self._h, byref(a)))
         return out
 
     def lr(self) -> float:  # ane/engine.go:358

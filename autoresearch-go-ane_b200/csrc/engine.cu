@@ -25,6 +25,7 @@
 #include "dp.h"
 #include "gemm.h"
 #include "kernels.h"
+#include "serving.h"
 
 namespace ane {
 
@@ -280,6 +281,7 @@ class EngineT final : public EngineBase {
   int eval_loss(const uint16_t* tokens, uint32_t n_seq, double* loss_sum, uint64_t* n_pos) override;
   int decode(const uint16_t* prompts, uint32_t n_seq, uint32_t prompt_len, uint32_t n_new, float temperature,
              const double* uniforms, uint16_t* out) override;
+  int generate(const ane_generate_args& g) override;
   int set_lr(float lr) override;
   float get_lr() override { return lr_; }
   int get_state(ane_state* s) override;
@@ -441,6 +443,8 @@ class EngineT final : public EngineBase {
   int layout_params();
   int alloc_buffers();
   int alloc_decode();
+  int alloc_generate(bool e4m3);
+  PagedKv generation_pages(int layer) const;
   void reserve_parts();
   int refresh_shadow();
   int forward(const uint16_t* d_tok, int B, int Tl, int pos0);
@@ -481,6 +485,19 @@ class EngineT final : public EngineBase {
   bool decoding_ = false;  // forward() runs one KV-cached decode step
   bool training_ = false;  // a backward pass follows forward(): halves are kept for it
   std::vector<T*> kcache_, vcache_;  // [B, S_, KV*hd] per layer (one block each for all layers), allocated by the first decode
+  // Generation over paged caches (generate(), bf16 engines): pages of kGenPage tokens for batch x seq, allocated by the first call of each
+  // type, keys of all layers and then values; a sequence's pages follow one another.
+  static constexpr int kGenPage = 64, kGenBiases = 1024;
+  const Batch* gen_batch_ = nullptr;  // forward() runs a part of a generation
+  int gen_max_new_ = 0;
+  bool gen_e4m3_ = false;
+  uint8_t *gen_bf16_ = nullptr, *gen_8bit_ = nullptr, *gen_work_ = nullptr;
+  float *gen_scales_ = nullptr, *gen_penalties_ = nullptr, *gen_bias_ = nullptr;
+  int *gen_table_ = nullptr, *gen_start_ = nullptr, *gen_pos_ = nullptr, *gen_tokens_ = nullptr, *gen_n_ = nullptr, *gen_prompt_ = nullptr,
+      *gen_mask_row_ = nullptr, *gen_bias_start_ = nullptr, *gen_bias_token_ = nullptr, *gen_choice_ = nullptr;
+  uint32_t* gen_mask_ = nullptr;
+  uint16_t *gen_next_ = nullptr, *gen_out_ = nullptr;
+  double* gen_u_ = nullptr;
   // scratch of the persistent decode kernel (bf16 engines)
   unsigned long long* dec_best_ = nullptr;
   double* dec_psum_ = nullptr;
@@ -1181,7 +1198,7 @@ int EngineT<T>::forward(const uint16_t* d_tok, int B, int Tl, int pos0) {
     rmsnorm_forward<T>(xs_[l], w_att, a.xn, a.rstd1, M, D_, stream_, blend);
     // llama arch, bf16, head_dim 64: the rotation of q and k happens on the fp32 accumulators in the epilogue
     static const bool no_fuse_rope = getenv("ANE_B200_NO_FUSE_ROPE") != nullptr;  // A/B measurements
-    const bool fused_rope = !kIsF32 && !qkv_f32_ && !isN_ && hd_ == 64 && !no_fuse_rope;
+    const bool fused_rope = !kIsF32 && !qkv_f32_ && !isN_ && hd_ == 64 && !no_fuse_rope && !gen_batch_;
     {
       GemmDesc g;
       g.A = a.xn; g.B = wop(s_qkv_[l].off); g.C = a.qkv;
@@ -1210,7 +1227,7 @@ int EngineT<T>::forward(const uint16_t* d_tok, int B, int Tl, int pos0) {
       ve_forward<float>((float*)a.qkv, xs_[l], d_tok, P_ + s_ve_embed_[l].off, P_ + s_ve_gate_[l].off, a.ve_act, M, D_,
                         H_, KV_, hd_, V_, stream_);
     }
-    if (!fused_rope) {
+    if (!fused_rope && !gen_batch_) {
       count_launch();
       if (fuse_hi) {
         rope_qknorm_forward_hd64((float*)a.qkv, (float*)a.qkpre, rope_cos_, rope_sin_, M, Tl, H_, KV_, isN_, pos0, qkvh_, stream_);
@@ -1226,7 +1243,18 @@ int EngineT<T>::forward(const uint16_t* d_tok, int B, int Tl, int pos0) {
                         H_, KV_, hd_, V_, stream_);
     }
     count_launch();
-    if (decoding_) {
+    if (gen_batch_) {
+      if constexpr (!kIsF32) {
+        // positions differ from sequence to sequence: the rotation happens on the way into the cache, that of q in place
+        const PagedKv kv = generation_pages(l);
+        bf16* qkv = (bf16*)a.qkv;
+        count_launch(2);  // attention may take a second one for joining
+        if ((rc = cuda_check(kv_append(kv, *gen_batch_, H_, qkv, QKVD_, qkv, QKVD_, rope_cos_, rope_sin_, S_, d_status_, stream_), "kv_append")) != 0 ||
+            (rc = cuda_check(kv_attention(kv, *gen_batch_, H_, qkv, QKVD_, (bf16*)a.att, QD_, gen_max_new_, 0, att_scale, gen_work_, d_status_,
+                                          stream_), "kv_attention")) != 0)
+          return rc;
+      }
+    } else if (decoding_) {
       // one new token per sequence: append its k|v to the cache and attend over positions 0..pos0
       kv_cache_append<T>((const T*)a.qkv, kcache_[l], vcache_[l], B, S_, pos0, H_, KV_, hd_, stream_);
       count_launch();
@@ -2322,6 +2350,220 @@ int EngineT<T>::decode(const uint16_t* prompts, uint32_t n_seq, uint32_t prompt_
   if ((rc = cuda_check(cudaMemcpyAsync(out, d_dec_out_, sizeof(uint16_t) * (size_t)B * n_new, cudaMemcpyDeviceToHost,
                                        stream_),
                        "decode download")) != 0)
+    return rc;
+  return check_device_status(nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Generation with prompts of different lengths, a paged cache of bf16 or 8 bits, and rules on the logits: the layer stack over all
+// prompts' tokens at once, then over one token of each sequence, with the serving kernels in the place of rotation, cache and attention.
+// ------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void generation_rows_kernel(const T* __restrict__ x, T* __restrict__ out, const int* __restrict__ start, int D) {
+  const T* from = x + (size_t)(start[blockIdx.x + 1] - 1) * D;  // a sequence's last row
+  for (int i = threadIdx.x; i < D; i += blockDim.x) out[(size_t)blockIdx.x * D + i] = from[i];
+}
+// The chosen tokens become the next pass' input, at the places behind the ones before.
+__global__ void generation_advance_kernel(const int* __restrict__ choice, uint16_t* __restrict__ next, uint16_t* __restrict__ out, int* __restrict__ tokens,
+                                          int* __restrict__ n, int* __restrict__ pos, int* __restrict__ start, int B, int n_new, int step, int S) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b > B) return;
+  start[b] = b;
+  if (b == B) return;
+  const int t = choice[b], at = n[b];
+  next[b] = (uint16_t)t;
+  out[(size_t)b * n_new + step] = (uint16_t)t;
+  tokens[(size_t)b * S + at] = t;
+  pos[b] = at;
+  n[b] = at + 1;
+}
+
+template <typename T>
+PagedKv EngineT<T>::generation_pages(int layer) const {
+  PagedKv kv;
+  const int slots = (S_ + kGenPage - 1) / kGenPage;
+  kv.e4m3 = gen_e4m3_;
+  kv.n_pages = B_ * slots; kv.page_size = kGenPage; kv.kv_heads = KV_; kv.head_dim = hd_;
+  kv.page_stride = (long long)KV_ * kGenPage * hd_;
+  const size_t layer_bytes = (size_t)kv.n_pages * kv.page_stride * (gen_e4m3_ ? 1 : 2), layer_scales = (size_t)kv.n_pages * KV_;
+  uint8_t* pages = gen_e4m3_ ? gen_8bit_ : gen_bf16_;
+  kv.k = pages + layer_bytes * layer;
+  kv.v = pages + layer_bytes * (L_ + layer);
+  kv.k_scale = gen_e4m3_ ? gen_scales_ + layer_scales * layer : nullptr;
+  kv.v_scale = gen_e4m3_ ? gen_scales_ + layer_scales * (L_ + layer) : nullptr;
+  kv.table = gen_table_; kv.table_pitch = slots;
+  return kv;
+}
+
+// All of it or, when memory runs out, none.
+template <typename T>
+int EngineT<T>::alloc_generate(bool e4m3) {
+  const size_t held = allocs_.size();
+  const int slots = (S_ + kGenPage - 1) / kGenPage;
+  const size_t pages = (size_t)B_ * slots, elements = 2 * pages * L_ * KV_ * kGenPage * hd_;
+  const bool first = gen_table_ == nullptr;
+  int dev_sms = 0;
+  cudaDeviceGetAttribute(&dev_sms, cudaDevAttrMultiProcessorCount, o_.device);
+  uint8_t *block = nullptr, *work = nullptr;
+  float *scales = nullptr, *pen = nullptr, *bias = nullptr;
+  int *table = nullptr, *start = nullptr, *pos = nullptr, *tokens = nullptr, *n = nullptr, *prompt = nullptr, *row = nullptr, *bs = nullptr,
+      *bt = nullptr, *choice = nullptr;
+  uint32_t* mask = nullptr;
+  uint16_t *next = nullptr, *out = nullptr;
+  double* u = nullptr;
+  const size_t B = B_, BS = (size_t)B_ * S_;
+  int r = dalloc(&block, elements * (e4m3 ? 1 : 2));
+  if (r == 0 && e4m3) r = dalloc(&scales, 2 * pages * L_ * KV_);
+  if (r == 0 && first &&
+      ((r = dalloc(&work, kv_attention_workspace(dev_sms, hd_))) != 0 || (r = dalloc(&pen, 3 * B)) != 0 || (r = dalloc(&bias, B * kGenBiases)) != 0 ||
+       (r = dalloc(&table, pages)) != 0 || (r = dalloc(&start, B + 1)) != 0 || (r = dalloc(&pos, B)) != 0 || (r = dalloc(&tokens, BS)) != 0 ||
+       (r = dalloc(&n, B)) != 0 || (r = dalloc(&prompt, B)) != 0 || (r = dalloc(&row, B)) != 0 || (r = dalloc(&bs, B + 1)) != 0 ||
+       (r = dalloc(&bt, B * kGenBiases)) != 0 || (r = dalloc(&choice, B)) != 0 || (r = dalloc(&mask, ((size_t)V_ + 31) / 32)) != 0 ||
+       (r = dalloc(&next, B)) != 0 || (r = dalloc(&out, BS)) != 0 || (r = dalloc(&u, BS)) != 0)) {
+  }
+  if (r == 0 && first) {
+    std::vector<int> pages_of(pages);
+    for (size_t i = 0; i < pages; ++i) pages_of[i] = (int)i;
+    r = cuda_check(cudaMemcpyAsync(table, pages_of.data(), sizeof(int) * pages, cudaMemcpyHostToDevice, stream_), "generation pages");
+    if (r == 0) r = cuda_check(cudaMemsetAsync(row, 0, sizeof(int) * B, stream_), "generation masks");
+    if (r == 0) r = cuda_check(cudaStreamSynchronize(stream_), "generation pages");
+  }
+  if (r != 0) {
+    for (; allocs_.size() > held; allocs_.pop_back()) cudaFree(allocs_.back());
+    cudaGetLastError();
+    return r;
+  }
+  (e4m3 ? gen_8bit_ : gen_bf16_) = block;
+  if (e4m3) gen_scales_ = scales;
+  if (first) {
+    gen_work_ = work; gen_penalties_ = pen; gen_bias_ = bias; gen_table_ = table; gen_start_ = start; gen_pos_ = pos; gen_tokens_ = tokens;
+    gen_n_ = n; gen_prompt_ = prompt; gen_mask_row_ = row; gen_bias_start_ = bs; gen_bias_token_ = bt; gen_choice_ = choice; gen_mask_ = mask;
+    gen_next_ = next; gen_out_ = out; gen_u_ = u;
+  }
+  return 0;
+}
+
+template <typename T>
+int EngineT<T>::generate(const ane_generate_args& g) {
+  std::lock_guard<std::mutex> call(in_call_);
+  if (isN_) return fail(ANE_ERR_STATE, "storiesane generate: KV-cache decoding is built for the llama-style architecture");
+  if (kIsF32 || qkv_f32_) return fail(ANE_ERR_STATE, "storiesane generate: paged caches are built for bf16 engines");
+  if (!kv_head_dim_supported(hd_)) return fail(ANE_ERR_STATE, "storiesane generate: head size must be 32, 48, 64, 96 or 128");
+  if (g.kv_dtype != ANE_KV_BF16 && g.kv_dtype != ANE_KV_E4M3) return fail(ANE_ERR_ARG, "storiesane generate: unknown kv_dtype");
+  const bool sampling = g.temperature > 1e-6f;
+  if (sampling && !g.uniforms) return fail(ANE_ERR_ARG, "storiesane generate: sampling needs one uniform draw per token");
+  if (!(g.repetition >= 0.f) || g.presence != g.presence || g.frequency != g.frequency)
+    return fail(ANE_ERR_ARG, "storiesane generate: bad penalties");
+  if (g.n_seq == 0 || (int64_t)g.n_seq > B_) return fail(ANE_ERR_ARG, "storiesane generate: n_seq must be in [1, batch]");
+  if (!g.prompts || !g.prompt_len || !g.out || (g.n_bias && (!g.bias_token || !g.bias))) return fail(ANE_ERR_ARG, "storiesane generate: null buffer");
+  if (g.n_bias > (uint32_t)kGenBiases) return fail(ANE_ERR_ARG, "storiesane generate: more than 1024 biases");
+  const int B = (int)g.n_seq, N = (int)g.n_new;
+  if (g.n_new == 0 || g.n_new > (uint32_t)S_) return fail(ANE_ERR_ARG, "storiesane generate: n_new must be in [1, seq)");
+  std::vector<int> start(B + 1, 0), prompt(B), zero(B, 0);
+  int longest = 0;
+  for (int b = 0; b < B; ++b) {
+    if (g.prompt_len[b] == 0 || g.prompt_len[b] > (uint32_t)(S_ - N)) return fail(ANE_ERR_ARG, "storiesane generate: prompt_len + n_new must fit the engine's seq");
+    prompt[b] = (int)g.prompt_len[b];
+    start[b + 1] = start[b] + prompt[b];
+    longest = std::max(longest, prompt[b]);
+  }
+  if (g.allowed) {
+    uint32_t any = 0;
+    for (int v = 0; v < V_; ++v) any |= g.allowed[v >> 5] >> (v & 31) & 1u;
+    if (!any) return fail(ANE_ERR_ARG, "storiesane generate: no token is allowed");
+  }
+  int rc;
+  if ((rc = cuda_check(cudaSetDevice(o_.device), "cudaSetDevice")) != 0) return rc;
+  gen_e4m3_ = g.kv_dtype == ANE_KV_E4M3;
+  if (!(gen_e4m3_ ? gen_8bit_ : gen_bf16_) && (rc = alloc_generate(gen_e4m3_)) != 0) return rc;
+
+  const int M = start[B];
+  auto up = [&](void* dst, const void* src, size_t bytes) { return cuda_check(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, stream_), "generation upload"); };
+  memcpy(h_in_, g.prompts, sizeof(uint16_t) * (size_t)M);
+  std::vector<int> tokens((size_t)B * S_, 0);
+  for (int b = 0; b < B; ++b)
+    for (int i = 0; i < prompt[b]; ++i) tokens[(size_t)b * S_ + i] = g.prompts[start[b] + i];
+  const bool penalise = (g.repetition != 0.f && g.repetition != 1.f) || g.presence != 0.f || g.frequency != 0.f;
+  if ((rc = up(d_in_, h_in_, sizeof(uint16_t) * (size_t)M)) != 0 || (rc = up(gen_start_, start.data(), sizeof(int) * (B + 1))) != 0 ||
+      (rc = up(gen_pos_, zero.data(), sizeof(int) * B)) != 0 || (rc = up(gen_n_, prompt.data(), sizeof(int) * B)) != 0 ||
+      (rc = up(gen_prompt_, prompt.data(), sizeof(int) * B)) != 0 || (rc = up(gen_tokens_, tokens.data(), sizeof(int) * tokens.size())) != 0)
+    return rc;
+  ane_logit_rules_args rules = {};
+  rules.struct_size = sizeof rules;
+  rules.dtype = ANE_DTYPE_F32;
+  rules.d_logits = rules.d_out = logits_;
+  rules.ld_logits = rules.ld_out = V_;
+  rules.rows = B;
+  rules.vocab = V_;
+  std::vector<float> pen(3 * (size_t)B), bias;
+  std::vector<int> bias_start(B + 1), bias_token;
+  if (penalise) {
+    for (int b = 0; b < B; ++b) {
+      pen[b] = g.repetition != 0.f ? g.repetition : 1.f;
+      pen[B + b] = g.presence;
+      pen[2 * B + b] = g.frequency;
+    }
+    if ((rc = up(gen_penalties_, pen.data(), sizeof(float) * pen.size())) != 0) return rc;
+    rules.d_tokens = gen_tokens_;
+    rules.d_n_tokens = gen_n_;
+    rules.d_n_prompt = gen_prompt_;
+    rules.ld_tokens = S_;
+    rules.d_repetition = gen_penalties_;
+    rules.d_presence = gen_penalties_ + B;
+    rules.d_frequency = gen_penalties_ + 2 * B;
+  }
+  if (g.n_bias) {
+    for (int b = 0; b < B; ++b) {
+      bias_start[b + 1] = bias_start[b] + (int)g.n_bias;
+      bias_token.insert(bias_token.end(), g.bias_token, g.bias_token + g.n_bias);
+      bias.insert(bias.end(), g.bias, g.bias + g.n_bias);
+    }
+    if ((rc = up(gen_bias_start_, bias_start.data(), sizeof(int) * bias_start.size())) != 0 ||
+        (rc = up(gen_bias_token_, bias_token.data(), sizeof(int) * bias_token.size())) != 0 || (rc = up(gen_bias_, bias.data(), sizeof(float) * bias.size())) != 0)
+      return rc;
+    rules.d_bias_start = gen_bias_start_;
+    rules.d_bias_token = gen_bias_token_;
+    rules.d_bias = gen_bias_;
+  }
+  if (g.allowed) {
+    if ((rc = up(gen_mask_, g.allowed, sizeof(uint32_t) * (((size_t)V_ + 31) / 32))) != 0) return rc;
+    rules.d_mask = gen_mask_;
+    rules.d_mask_row = gen_mask_row_;
+    rules.n_masks = 1;
+    rules.ld_mask = (V_ + 31) / 32;
+  }
+  const bool ruled = penalise || g.n_bias || g.allowed;
+  if (sampling && (rc = up(gen_u_, g.uniforms, sizeof(double) * (size_t)B * N)) != 0) return rc;
+
+  Batch batch = {gen_start_, gen_pos_, B, M};
+  for (int step = 0; step < N; ++step) {
+    const T* last = xnf_;  // the rows that logits are wanted of
+    batch.n_tokens = step == 0 ? M : B;
+    gen_batch_ = &batch;
+    gen_max_new_ = step == 0 ? longest : 1;
+    rc = step == 0 ? forward(d_in_, 1, M, 0) : forward(gen_next_, B, 1, 0);
+    gen_batch_ = nullptr;
+    if (rc != 0) return rc;
+    if (step == 0) {
+      last = acts_[0].xn;
+      count_launch();
+      generation_rows_kernel<T><<<B, 128, 0, stream_>>>(xnf_, acts_[0].xn, gen_start_, D_);
+    }
+    GemmDesc d;
+    d.A = last; d.B = wop(s_embed_.off); d.C = logits_;
+    d.M = B; d.N = V_; d.K = D_; d.lda = D_; d.ldb = D_; d.ldc = V_; d.out = GEMM_OUT_F32;
+    count_launch();
+    if ((rc = gemm(d)) != 0) return rc;
+    if (ruled) {
+      count_launch();
+      if ((rc = cuda_check(logit_rules(rules, d_status_, stream_), "logit_rules")) != 0) return rc;
+    }
+    count_launch(2);
+    sample_rows(logits_, gen_u_ + (size_t)step * B, sampling ? g.temperature : 0.f, gen_choice_, B, V_, stream_);
+    generation_advance_kernel<<<(B + 128) / 128, 128, 0, stream_>>>(gen_choice_, gen_next_, gen_out_, gen_tokens_, gen_n_, gen_pos_, gen_start_, B, N,
+                                                                    step, S_);
+  }
+  if ((rc = cuda_check(cudaMemcpyAsync(g.out, gen_out_, sizeof(uint16_t) * (size_t)B * N, cudaMemcpyDeviceToHost, stream_), "generation download")) != 0)
     return rc;
   return check_device_status(nullptr);
 }

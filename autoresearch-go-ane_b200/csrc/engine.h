@@ -22,6 +22,7 @@ class EngineBase {
   virtual int eval_loss(const uint16_t* tokens, uint32_t n_seq, double* loss_sum, uint64_t* n_pos) = 0;
   virtual int decode(const uint16_t* prompts, uint32_t n_seq, uint32_t prompt_len, uint32_t n_new, float temperature,
                      const double* uniforms, uint16_t* out) = 0;
+  virtual int generate(const ane_generate_args& g) = 0;
   virtual int set_lr(float lr) = 0;
   virtual float get_lr() = 0;
   virtual int get_state(ane_state* s) = 0;

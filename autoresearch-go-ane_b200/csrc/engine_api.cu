@@ -13,6 +13,7 @@ struct ane_engine {
 // The Go and Python bindings mirror these layouts field by field.
 static_assert(sizeof(ane_options) == 168, "ane_options layout changed: update the bindings");
 static_assert(sizeof(ane_step_result) == 112, "ane_step_result layout changed: update the bindings");
+static_assert(sizeof(ane_generate_args) == 96, "ane_generate_args layout changed: update the bindings");
 static_assert(sizeof(ane_state) == 56, "ane_state layout changed: update the bindings");
 
 static thread_local std::string g_api_err;
@@ -135,6 +136,14 @@ int32_t ane_decode_sample(ane_engine* e, const uint16_t* prompts, uint32_t n_seq
     return ANE_ERR_ARG;
   }
   return e->impl->decode(prompts, n_seq, prompt_len, n_new, temperature, uniforms, out);
+}
+int32_t ane_generate(ane_engine* e, const ane_generate_args* args) {
+  ENGINE_OR_FAIL(e, "generate");
+  if (!args || args->struct_size != sizeof(ane_generate_args)) {
+    g_api_err = "storiesane generate: bad struct_size";
+    return ANE_ERR_ARG;
+  }
+  return e->impl->generate(*args);
 }
 int32_t ane_set_lr(ane_engine* e, float lr) {
   ENGINE_OR_FAIL(e, "set lr");

@@ -349,6 +349,30 @@ int32_t ane_decode_greedy(ane_engine* e, const uint16_t* prompts, uint32_t n_seq
  * <= 1e-6 is the argmax and ignores uniforms. */
 int32_t ane_decode_sample(ane_engine* e, const uint16_t* prompts, uint32_t n_seq, uint32_t prompt_len, uint32_t n_new,
                           float temperature, const double* uniforms, uint16_t* out);
+
+/* Generation over paged caches, on ane_op_kv_append, ane_op_kv_attention and ane_op_logit_rules: prompts of different lengths, keys and
+ * values in bf16 or 8 bits, penalties for repeated tokens, biases and a mask of allowed tokens, greedy or sampled as above (bf16 engines of
+ * the llama-style architecture, head size 32, 48, 64, 96 or 128; n_seq <= batch, each prompt_len + n_new <= seq).  The first call of
+ * each kv_dtype takes the memory for batch x seq tokens.  No counterpart in the reference. */
+typedef struct ane_generate_args {
+  uint32_t struct_size;
+  uint32_t n_seq;
+  const uint16_t* prompts;    /* the sequences' prompts one after the other */
+  const uint32_t* prompt_len; /* [n_seq] */
+  uint32_t n_new;
+  int32_t kv_dtype;           /* ANE_KV_BF16 or ANE_KV_E4M3 */
+  float temperature;          /* <= 1e-6: argmax */
+  float repetition;           /* penalties as in ane_op_logit_rules; 0 (and 1 for this one): none */
+  float presence, frequency;
+  const double* uniforms;     /* [n_new][n_seq] draws, as in ane_decode_sample */
+  const uint32_t* allowed;    /* bit v % 32 of word v / 32 allows token v, for all sequences; NULL: all */
+  const int32_t* bias_token;  /* [n_bias] biases for all sequences, up to 1024 */
+  const float* bias;
+  uint32_t n_bias;
+  uint32_t pad_;
+  uint16_t* out;              /* [n_seq][n_new] */
+} ane_generate_args;
+int32_t ane_generate(ane_engine* e, const ane_generate_args* args);
 int32_t ane_set_lr(ane_engine* e, float lr);   /* ane/engine.go:366 */
 float ane_get_lr(ane_engine* e);               /* ane/engine.go:358 */
 int32_t ane_get_state(ane_engine* e, ane_state* out);       /* ane/engine.go:498 */
