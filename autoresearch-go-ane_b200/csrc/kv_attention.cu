@@ -229,17 +229,19 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
   __shared__ int sums[kWarps];
   __shared__ int4 at, span;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // A thread has some sequences, or, where those are few and have many tiles of rows, a part of one's: 2^split threads a sequence.
   const int per = (a.batch.n_seq + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, a.batch.n_seq), b1 = min(b0 + per, a.batch.n_seq);
+  const int split = per > 1 || (F::kSplit && a.one_tile) ? 0 : 31 - __clz(kThreads / a.batch.n_seq), part = tid & ((1 << split) - 1);
+  const int b0 = min((tid >> split) * per, a.batch.n_seq), b1 = min(b0 + per, a.batch.n_seq);
   Span s = {0, 0, 0};  // of the thread's only sequence, mostly
   // what(tiles of an item) of all items of a KV head of the thread's sequences, until it says stop
   auto each = [&](auto what) {
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       if (per > 1) s = span_of(a.batch, b, a.capacity, a.max_new, a.status);
-      const int mts = row_tiles<F>(a, s);
+      const int mts = row_tiles<F>(a, s), each_mts = (mts + (1 << split) - 1) >> split, mt1 = min(mts, (part + 1) * each_mts);
 #pragma unroll 1
-      for (int mt = 0; mt < mts; ++mt)
+      for (int mt = part * each_mts; mt < mt1; ++mt)
         if (what(b, mt, range_of<F>(a, s, mt).template tiles<F>())) return;
     }
   };
@@ -998,46 +1000,60 @@ __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int 
       make_uint2(pack<false>(o.x * by, o.y * by), pack<false>(o.z * by, o.w * by));
 }
 
-// The same by a warp, for a few parts.
+// The same of eight rows from `row` on by a block, for at most kFew parts: a row takes as many lanes as it has groups of four columns, rounded up to
+// a power of two.
+constexpr int kFew = 6;
 template <int HD, int kRows>
-__device__ __forceinline__ void join_row_by_warp(const Attn& a, int cta, int4 item, int row) {
+__device__ __forceinline__ void join_rows(const Attn& a, int cta, int4 item, int row0) {
+  constexpr int lanes = HD <= 32 ? 8 : HD <= 64 ? 16 : 32;
   const Span s = span_of(a.batch, item.x, INT32_MAX, INT32_MAX, a.status);
-  const int at = item.y * kRows + row, parts = item.w, lane = threadIdx.x & 31;
-  if (at >= s.n * a.group) return;
-  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row; };
-  float2 st = lane < parts ? a.stats[slot(lane)] : make_float2(-INFINITY, 0.f);
-  const float m = warp_max(st.x), f = exp2_fast(st.x - (m == -INFINITY ? 0.f : m)), l = warp_sum(st.y * f), by = l == 0.f ? 0.f : 1.f / l;
-  const int t = a.by_group(at), hd = at - t * a.group;
-  bf16* out = a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(item.z * a.group + hd) * HD;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float fi = __shfl_sync(0xffffffffu, f, i) * by;
-    if (lane * 4 >= HD) continue;
-    const float4 v = *reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4);
-    o.x = fmaf(v.x, fi, o.x); o.y = fmaf(v.y, fi, o.y); o.z = fmaf(v.z, fi, o.z); o.w = fmaf(v.w, fi, o.w);
+  const int parts = item.w, lane = threadIdx.x % lanes, row = row0 + threadIdx.x / lanes, at = item.y * kRows + row;
+  if (threadIdx.x / lanes >= 8 || row >= kRows || at >= s.n * a.group) return;
+  const bool mine = lane * 4 < HD;
+  float2 st[kFew];
+  float4 v[kFew];
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    // part i: the first CTA's second slot, then the first slot of each
+    const size_t slot = (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row;
+    st[i] = i < parts ? a.stats[slot] : make_float2(-INFINITY, 0.f);
+    v[i] = i < parts && mine ? *reinterpret_cast<const float4*>(a.part + slot * HD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  if (lane * 4 < HD) *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack<false>(o.x, o.y), pack<false>(o.z, o.w));
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) m = fmaxf(m, st[i].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kFew; ++i) {
+    const float f = exp2_fast(st[i].x - base);
+    l = fmaf(st[i].y, f, l);
+    o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
+  }
+  const float by = l == 0.f ? 0.f : 1.f / l;
+  const int t = a.by_group(at), hd = at - t * a.group;
+  if (mine)
+    *reinterpret_cast<uint2*>(a.out + (size_t)(s.row + t) * a.ld_out + (size_t)(item.z * a.group + hd) * HD + lane * 4) =
+        make_uint2(pack<false>(o.x * by, o.y * by), pack<false>(o.z * by, o.w * by));
 }
 
 // Rows of shared items, task t: row t % rows of the item that begins in CTA t / rows.  Most CTAs of the first kernel begin none: 32 tasks are
-// looked at together.  Items of up to kFew parts take a warp a row, eight rows from every eighth task, others a block.  The
-// grid's size is odd where a block has several tasks, so that those are spread evenly.
+// looked at together.  Items of up to kFew parts take a part of a block a row, eight rows from every eighth task, others a block.
+// The grid's size is odd where a block has several tasks, so that those are spread evenly.
 template <int HD, int kRows>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int ctas, int rows) {
-  constexpr int kFew = 6, kWarps = kJoinThreads / 32;
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, tasks = ctas * rows;  // this block's: blockIdx.x, + gridDim.x, ...
   for (int t0 = blockIdx.x; t0 < tasks; t0 += 32 * gridDim.x) {
     const int mine = t0 + lane * (int)gridDim.x, my_cta = mine / rows, my_row = mine - my_cta * rows;
     const int4 item = mine < tasks ? a.head[my_cta] : make_int4(-1, 0, 0, 0);
-    for (uint32_t left = __ballot_sync(0xffffffffu, item.x >= 0 && (item.w > kFew || my_row % kWarps == 0)); left; left &= left - 1) {
+    for (uint32_t left = __ballot_sync(0xffffffffu, item.x >= 0 && (item.w > kFew || my_row % 8 == 0)); left; left &= left - 1) {
       const int from = __ffs(left) - 1, cta = __shfl_sync(0xffffffffu, my_cta, from), row = __shfl_sync(0xffffffffu, my_row, from);
       const int4 one = make_int4(__shfl_sync(0xffffffffu, item.x, from), __shfl_sync(0xffffffffu, item.y, from),
                                  __shfl_sync(0xffffffffu, item.z, from), __shfl_sync(0xffffffffu, item.w, from));
       if (one.w <= kFew) {
-        if (row + (int)(threadIdx.x >> 5) < rows) join_row_by_warp<HD, kRows>(a, cta, one, row + (threadIdx.x >> 5));
+        join_rows<HD, kRows>(a, cta, one, row);
         continue;
       }
       join_row<HD, kRows>(a, cta, one, row);
@@ -1072,7 +1088,7 @@ cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
   cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(F::kThreads), a.stages * F::kStage, s, a);
   if (e != cudaSuccess || !may_share) return e;
   const int rows = (int)min((long long)kRows, (long long)a.max_new * a.group);
-  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, 4ll * sms - 1)), dim3(kJoinThreads), 0, s, a, ctas, rows);
+  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, (kRows > 32 ? 8ll : 4ll) * sms - 1)), dim3(kJoinThreads), 0, s, a, ctas, rows);
 }
 
 // Which form, by the rows of one KV head that a sequence has at most.  Tiles of few rows that all warps share leave no warp without rows and
