@@ -2539,11 +2539,15 @@ int EngineT<T>::generate(const ane_generate_args& g) {
   for (int step = 0; step < N; ++step) {
     const T* last = xnf_;  // the rows that logits are wanted of
     batch.n_tokens = step == 0 ? M : B;
-    gen_batch_ = &batch;
     gen_max_new_ = step == 0 ? longest : 1;
-    rc = step == 0 ? forward(d_in_, 1, M, 0) : forward(gen_next_, B, 1, 0);
-    gen_batch_ = nullptr;
-    if (rc != 0) return rc;
+    {
+      struct Scope {
+        const Batch*& now;
+        ~Scope() { now = nullptr; }
+      } scope{gen_batch_};
+      gen_batch_ = &batch;
+      if ((rc = step == 0 ? forward(d_in_, 1, M, 0) : forward(gen_next_, B, 1, 0)) != 0) return rc;
+    }
     if (step == 0) {
       last = acts_[0].xn;
       count_launch();

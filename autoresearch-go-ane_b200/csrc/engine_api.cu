@@ -143,7 +143,12 @@ int32_t ane_generate(ane_engine* e, const ane_generate_args* args) {
     g_api_err = "storiesane generate: bad struct_size";
     return ANE_ERR_ARG;
   }
-  return e->impl->generate(*args);
+  try {
+    return e->impl->generate(*args);
+  } catch (...) {  // no memory on the host
+    g_api_err = "storiesane generate: out of memory";
+    return ANE_ERR_STATE;
+  }
 }
 int32_t ane_set_lr(ane_engine* e, float lr) {
   ENGINE_OR_FAIL(e, "set lr");

@@ -341,7 +341,7 @@ struct Rows {  // 8 * NB rows of queries
   // and what brings products to scores in log2
   float base[NB][2], limit[NB][2], l[NB][2], mult[NB][2];
   int pos[NB][2];                         // their positions; -1: no such row
-  float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = kPScale / v_ref
+  float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = 1 / v_ref, which is finite
 };
 
 template <int HD, int NB>
@@ -416,7 +416,7 @@ __device__ __forceinline__ void begin_rows(const Attn& a, const Item& it, int ro
     for (int y = 0; y < HD / 16; ++y) r.o[n][y][0] = r.o[n][y][1] = r.o[n][y][2] = r.o[n][y][3] = 0.f;
   }
   r.v_ref = kLowest;
-  r.v_inv = kPScale / kLowest;
+  r.v_inv = 1.f / kLowest;
 }
 
 // Whether one of a word's values is infinite or NaN.
@@ -514,7 +514,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
     if (most > r.v_ref) {  // statistics keep their unit, the output changes to the new one
       const float by = r.v_ref / most;
       r.v_ref = most;
-      r.v_inv = kPScale / most;
+      r.v_inv = 1.f / most;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -523,7 +523,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
           for (int i = 0; i < 4; ++i) r.o[n][y][i] *= by;
     }
 #pragma unroll
-    for (int k = 0; k < KG; ++k) into[k] = scale[k].y * r.v_inv;
+    for (int k = 0; k < KG; ++k) into[k] = scale[k].y * r.v_inv * kPScale;
   }
   uint32_t p[KG][NB][2], rest[kRest ? KG : 1][NB][2];
   bool above = false;

@@ -345,6 +345,7 @@ int32_t ane_op_kv_append(const ane_kv_append_args* a) {
     const cudaError_t e = kv_append(paged_kv(c), batch, a->n_heads, reinterpret_cast<const bf16*>(a->d_qkv), a->ld_qkv,
                                     reinterpret_cast<bf16*>(a->d_q), a->ld_q, a->d_cos, a->d_sin, a->n_positions, status,
                                     reinterpret_cast<cudaStream_t>(a->stream));
+    if (e == cudaErrorInvalidValue) return *fault = "too much for one call", ANE_ERR_ARG;
     return e == cudaSuccess ? 0 : cuda_fail(e, "ane_op_kv_append");
   });
 }
@@ -387,6 +388,7 @@ int32_t ane_op_kv_attention(const ane_kv_attention_args* a) {
     const cudaError_t e = kv_attention(paged_kv(c), batch, a->n_heads, reinterpret_cast<const bf16*>(a->d_q), a->ld_q,
                                        reinterpret_cast<bf16*>(a->d_out), a->ld_out, a->max_new, a->window, a->scale, a->d_workspace,
                                        status, reinterpret_cast<cudaStream_t>(a->stream));
+    if (e == cudaErrorInvalidValue) return *fault = "too much for one call", ANE_ERR_ARG;
     return e == cudaSuccess ? 0 : cuda_fail(e, "ane_op_kv_attention");
   });
 }

@@ -182,13 +182,14 @@ int32_t ane_op_kv_append(const ane_kv_append_args* args);
 
 /* Attention of new tokens over their sequences' caches, the new tokens' own keys included (append first): the token at
  * position p sees positions 0 .. p, with a window only the last `window` of them.  One token a sequence or many.  Softmax statistics
- * and sums in fp32, probabilities enter their product in 16 bits.  Results are the same from call to call. */
+ * and sums in fp32, probabilities enter their product in 16 bits (of up to 16 query heads' rows a KV head, with what that leaves of them).
+ * Results are the same from call to call. */
 typedef struct ane_kv_attention_args {
   uint32_t struct_size;
   int32_t n_heads;
   const ane_kv_cache* cache;
   const void* d_q;           /* bf16 [n_tokens][ld_q], n_heads * head_dim columns, rotated */
-  void* d_out;               /* bf16 [n_tokens][ld_out] */
+  void* d_out;               /* bf16 [n_tokens][ld_out]; not d_q */
   int32_t ld_q, ld_out;      /* multiples of 8 */
   const int32_t* d_seq_start;
   const int32_t* d_pos;

@@ -280,6 +280,57 @@ def test_attention_scales_of_any_size_and_mixed():
     check_attention("e4m3", 4, 2, 64, 16, [1], [1999], cache=cache)
 
 
+@pytest.mark.parametrize("new", [1, 40, 100])
+def test_attention_pages_of_zeros_and_of_the_smallest_values(new):
+    # the scale of a page of zeros is 2^-126, the smallest that appending gives
+    heads, kv, hd, n = 2, 1, 64, 200 + new
+    cache = Cache([n], kv, hd, 16, "e4m3", fill=False)
+    qkv = torch.zeros(n, (heads + 2) * hd, dtype=torch.bfloat16, device="cuda")
+    qkv[:, :heads * hd] = 1.0
+    start, pos = i32([0, n]), i32([0])
+    append(cache, heads, qkv, None, start, pos, None, None)
+    q = qkv[200:, :heads * hd].contiguous()
+    out = torch.full_like(q, 7.0)
+    attention(cache, heads, q, out, i32([0, new]), i32([200]), new)
+    assert (out == 0).all()
+    tiny = 2.0 ** -125  # 1 or 2 in units of the scale: a bf16 and an e4m3 number
+    qkv[:, (heads + 1) * hd:] = tiny
+    append(cache, heads, qkv, None, start, pos, None, None)
+    attention(cache, heads, q, out, i32([0, new]), i32([200]), new)
+    assert status() == 0
+    assert ((out.double() / tiny - 1).abs() <= 2.0 ** -7).all()  # equal probabilities in 16 bits and their sums, rounded to bf16
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_sequences_may_share_full_pages(kind):
+    heads, kv, hd, page = 4, 2, 64, 16
+    cache = Cache([100, 100, 100], kv, hd, page, kind, seed=6)
+    for b in (1, 2):  # three sequences with the same first 64 tokens
+        for i in range(4):
+            cache.table_host[b][i] = cache.table_host[0][i]
+    cache.table = i32(cache.table_host)
+    check_attention(kind, heads, kv, hd, page, [1, 3, 20], [70, 64, 66], cache=cache)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_streams_at_once(kind):
+    heads, kv, hd = 8, 2, 64
+    caches = [Cache([9000, 3000], kv, hd, 64, kind, seed=i) for i in range(2)]
+    q = [torch.randn(2, heads * hd, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).cuda() for i in range(2)]
+    start, pos = i32([0, 1, 2]), i32([8999, 2999])
+    want = [torch.empty_like(x) for x in q]
+    for i in range(2):
+        attention(caches[i], heads, q[i], want[i], start, pos, 1)
+    works, streams = [workspace(heads, kv, hd) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.empty_like(x) for _ in range(20)] for x in q]
+    torch.cuda.synchronize()
+    for k in range(20):
+        for i in range(2):
+            attention(caches[i], heads, q[i], got[i][k], start, pos, 1, work=works[i], stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new", [1, 4, 40])
 def test_attention_does_not_see_infinite_values_ahead(kind, new):
