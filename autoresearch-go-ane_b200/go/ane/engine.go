@@ -152,6 +152,7 @@ var (
 	cTensorSize func(e uintptr, id, layer uint32) int64
 	cDecode     func(e uintptr, prompts *uint16, nSeq, promptLen, nNew uint32, temperature float32, uniforms *float64, out *uint16) int32
 	cReseed     func(e uintptr, seed int64) int32
+	cGenerate   func(e uintptr, args *cGenerateArgs) int32
 )
 
 func load() error {
@@ -183,6 +184,7 @@ func load() error {
 		purego.RegisterLibFunc(&cTensorSize, lib, "ane_tensor_size")
 		purego.RegisterLibFunc(&cDecode, lib, "ane_decode_sample")
 		purego.RegisterLibFunc(&cReseed, lib, "ane_reseed")
+		purego.RegisterLibFunc(&cGenerate, lib, "ane_generate")
 	})
 	return loadErr
 }
@@ -412,6 +414,106 @@ func (e *Engine) EvalLoss(tokens []uint16) (float64, int, error) {
 		return 0, 0, e.err("eval loss", rc)
 	}
 	return sum, int(n), nil
+}
+
+// cGenerateArgs mirrors ane_generate_args (include/ane_b200.h).
+type cGenerateArgs struct {
+	structSize, nSeq                             uint32
+	prompts                                      *uint16
+	promptLen                                    *uint32
+	nNew                                         uint32
+	kvDtype                                      int32
+	temperature, repetition, presence, frequency float32
+	uniforms                                     *float64
+	allowed                                      *uint32
+	biasToken                                    *int32
+	bias                                         *float32
+	nBias, pad                                   uint32
+	out                                          *uint16
+}
+
+// PagedOptions says how GeneratePaged chooses tokens and keeps keys and values.  Its zero value is greedy generation with a bf16 cache.
+type PagedOptions struct {
+	KV8Bit                          bool // e4m3 with a scale for each page and head instead of bf16
+	Temperature                     float32
+	Repetition, Presence, Frequency float32         // penalties for repeated tokens; 0 (and 1 for Repetition): none
+	Bias                            map[int32]float32 // added to the logits of tokens
+	Allowed                         []uint32          // bit v%32 of word v/32 allows token v; nil: all
+}
+
+// GeneratePaged continues prompts of different lengths by nNew tokens each over a paged KV cache (ane_generate): the result has a row for
+// each prompt.  rng is needed when sampling.
+func (e *Engine) GeneratePaged(rng *rand.Rand, prompts [][]uint16, nNew int, o PagedOptions) ([][]uint16, error) {
+	if e == nil || e.h == 0 {
+		return nil, fmt.Errorf("storiesane generate: engine is closed")
+	}
+	if len(prompts) == 0 || nNew <= 0 {
+		return nil, fmt.Errorf("storiesane generate: prompts=%d nNew=%d", len(prompts), nNew)
+	}
+	if o.Allowed != nil && len(o.Allowed) != (e.vocab+31)/32 {
+		return nil, fmt.Errorf("storiesane generate: allowed words=%d want=%d", len(o.Allowed), (e.vocab+31)/32)
+	}
+	var flat []uint16
+	lens := make([]uint32, len(prompts))
+	for i, p := range prompts {
+		flat = append(flat, p...)
+		lens[i] = uint32(len(p))
+	}
+	out := make([]uint16, len(prompts)*nNew)
+	a := cGenerateArgs{nSeq: uint32(len(prompts)), prompts: unsafe.SliceData(flat), promptLen: unsafe.SliceData(lens), nNew: uint32(nNew),
+		temperature: o.Temperature, repetition: o.Repetition, presence: o.Presence, frequency: o.Frequency,
+		allowed: unsafe.SliceData(o.Allowed), out: unsafe.SliceData(out)}
+	a.structSize = uint32(unsafe.Sizeof(a))
+	if o.KV8Bit {
+		a.kvDtype = 1
+	}
+	var draws []float64
+	if o.Temperature > 1e-6 {
+		if rng == nil {
+			return nil, fmt.Errorf("storiesane generate: sampling needs a rand source")
+		}
+		draws = make([]float64, len(out))
+		for i := range draws {
+			draws[i] = rng.Float64()
+		}
+		a.uniforms = unsafe.SliceData(draws)
+	}
+	var biasTokens []int32
+	var biases []float32
+	for t, b := range o.Bias {
+		biasTokens, biases = append(biasTokens, t), append(biases, b)
+	}
+	if len(biases) > 0 {
+		a.biasToken, a.bias, a.nBias = unsafe.SliceData(biasTokens), unsafe.SliceData(biases), uint32(len(biases))
+	}
+	// the structure holds pointers to Go memory for the length of the call only
+	var pin runtime.Pinner
+	defer pin.Unpin()
+	pin.Pin(&lens[0])
+	pin.Pin(&out[0])
+	if len(flat) > 0 {
+		pin.Pin(&flat[0])
+	}
+	if len(draws) > 0 {
+		pin.Pin(&draws[0])
+	}
+	if len(o.Allowed) > 0 {
+		pin.Pin(&o.Allowed[0])
+	}
+	if len(biases) > 0 {
+		pin.Pin(&biasTokens[0])
+		pin.Pin(&biases[0])
+	}
+	rc := cGenerate(e.h, &a)
+	runtime.KeepAlive(&a)
+	if rc != 0 {
+		return nil, e.err("generate", rc)
+	}
+	rows := make([][]uint16, len(prompts))
+	for i := range rows {
+		rows[i] = out[i*nNew : (i+1)*nNew : (i+1)*nNew]
+	}
+	return rows, nil
 }
 
 // Generate is additive: KV-cached generation for nSeq prompts of equal length laid out back to back.
