@@ -53,12 +53,14 @@ struct Layout {
   static constexpr int VV = RB % 128 == 0 ? 16 : RB % 64 == 0 ? 8 : RB % 32 == 0 ? 4 : 2;  // of V rows
 };
 
-// kSplit: eight warps share 8 * NB rows and take an eighth of the keys each; otherwise each of four has 8 * NB rows and takes all keys of a tile.
+// kSplit: the warps share 8 * NB rows and take a part of the keys each; otherwise each of four has 8 * NB rows and takes all keys of a tile.
+// Eight warps, but six where 8-bit pages and 128 * 8 outputs a warp do not fit the 128 registers that two CTAs of eight leave: 64 sequences of
+// 8192 tokens with heads of 128 take 118 us (5.7 TB/s) with 168 registers, 126 us with 128 and spills (heads of 64 and 16 rows: 166 and 168).
 // kGroups: times 16 keys that a warp takes at once.  More keys share their softmax's maximum, exchanges and loop, fewer leave the ring room
 // for more stages.
 template <int HD_, bool F8_, int NB_, bool kSplit_>
 struct Form {
-  static constexpr int HD = HD_, NB = NB_, kWarps = kSplit_ ? 8 : 4;
+  static constexpr int HD = HD_, NB = NB_, kWarps = kSplit_ ? (F8_ && HD_ * NB_ == 128 && NB_ <= 2 ? 6 : 8) : 4;
   static constexpr bool F8 = F8_, kSplit = kSplit_;
   using L = Layout<HD, F8>;
   static constexpr int kGroups = kSplit ? (L::RB <= 64 && NB == 1 ? 2 : 1) : 2;
@@ -109,6 +111,18 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same onto zeros.
+template <bool F8>
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F8)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {  // the low and the high two bytes
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
@@ -453,15 +467,12 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
     const char* ks = ring + k * 2 * L::GB;
     scale[k] = F8 ? scales[k] : make_float2(1.f, 1.f);
     float even[NB][4];  // a second chain of products, half as long each
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[k][n][i] = even[n][i] = 0.f;
     auto products = [&](const uint32_t (&a)[4], int step) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        if (kChains == 2 && step % 2 == 0) mma<F8>(even[n], a, r.q[n][step][0], r.q[n][step][1]);
-        else mma<F8>(s[k][n], a, r.q[n][step][0], r.q[n][step][1]);
+        float(&d)[4] = kChains == 2 && step % 2 == 1 ? even[n] : s[k][n];
+        if (step < kChains) mma_first<F8>(d, a, r.q[n][step][0], r.q[n][step][1]);
+        else mma<F8>(d, a, r.q[n][step][0], r.q[n][step][1]);
       }
     };
     if (F8) {
