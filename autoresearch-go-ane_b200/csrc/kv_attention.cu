@@ -1,14 +1,14 @@
 // Attention of new tokens over a paged KV cache (ane_op_kv_attention).
 //
 // The query heads of a KV head share its keys, so they are rows of one product: row r of a KV head's queries is token r / group,
-// head r % group.  Products are m16n8k16 on mma.sync: single tokens are bound by the bytes of the cache, and their
+// head r % group.  Few rows take m16n8k16 on mma.sync: single tokens are bound by the bytes of the cache, and their
 // products take a fraction of the time that the operands need to arrive.
 //
-//   few rows (up to 16 a KV head): a CTA holds 8 or 16 rows; its eight warps take 16 of every 128 keys each, with softmax
-//     statistics of their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
-//   many rows: a CTA holds 64 or 128 rows, a warp a quarter of them, and all warps go over all keys.
+//   few rows (up to 32 a KV head): a CTA holds 8, 16 or 32 rows; its warps take 16 of every 96 or 128 keys each, with softmax statistics
+//     of their own, joined at the end.  No barrier in the loop: every warp waits for its own copies only.
+//   many rows: 128 rows a CTA on tcgen05, see kv_attention_tc.cuh.
 //
-// Keys and values come by cp.async into a ring of stages of 64 keys.  8-bit ones stay 8-bit until they are in registers, where they
+// Keys and values come by cp.async into a ring of stages.  8-bit ones stay 8-bit until they are in registers, where they
 // become f16, which holds e4m3 exactly: queries are brought to f16 by a power of two per row, scales of keys go onto the
 // scores, scales of values onto the probabilities.
 //
@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "gemm_tc.cuh"
 #include "serving.h"
 
 namespace ane {
@@ -53,29 +54,29 @@ struct Layout {
   static constexpr int VV = RB % 128 == 0 ? 16 : RB % 64 == 0 ? 8 : RB % 32 == 0 ? 4 : 2;  // of V rows
 };
 
-// kSplit: the warps share 8 * NB rows and take a part of the keys each; otherwise each of four has 8 * NB rows and takes all keys of a tile.
+// A form for few rows: the warps share 8 * NB rows and take a part of the keys each, so that no warp is without rows.
 // Eight warps, but six where 8-bit pages and 128 * 8 outputs a warp do not fit the 128 registers that two CTAs of eight leave: 64 sequences of
 // 8192 tokens with heads of 128 take 118 us (5.7 TB/s) with 168 registers, 126 us with 128 and spills (heads of 64 and 16 rows: 166 and 168).
 // kGroups: times 16 keys that a warp takes at once.  More keys share their softmax's maximum, exchanges and loop, fewer leave the ring room
 // for more stages.
-template <int HD_, bool F8_, int NB_, bool kSplit_>
+template <int HD_, bool F8_, int NB_>
 struct Form {
-  static constexpr int HD = HD_, NB = NB_, kWarps = kSplit_ ? (F8_ && HD_ * NB_ == 128 && NB_ <= 2 ? 6 : 8) : 4;
-  static constexpr bool F8 = F8_, kSplit = kSplit_;
+  static constexpr int HD = HD_, NB = NB_, kWarps = F8_ && HD_ * NB_ == 128 && NB_ <= 2 ? 6 : 8;
+  static constexpr bool F8 = F8_, kSplit = true;
   using L = Layout<HD, F8>;
-  static constexpr int kGroups = kSplit ? (L::RB <= 64 && NB == 1 ? 2 : 1) : 2;
-  // groups of 16 keys of a tile that a warp fetches; the ring has to hold the outputs of kSplit's warps
-  static constexpr int kLoads = kSplit ? (kGroups * 3 * L::ES < NB ? 2 : kGroups) : L::RB <= 128 ? kGroups : 1;
-  static constexpr int kThreads = 32 * kWarps, kTile = kGroup * kWarps * kLoads;
-  static constexpr int kRows = kSplit ? 8 * NB : 8 * NB * kWarps;
+  static constexpr int kGroups = L::RB <= 64 && NB == 1 ? 2 : 1;
+  // groups of 16 keys of a tile that a warp fetches; the ring has to hold the warps' outputs
+  static constexpr int kLoads = kGroups * 3 * L::ES < NB ? 2 : kGroups;
+  static constexpr int kThreads = 32 * kWarps, kTile = kGroup * kWarps * kLoads, kRows = 8 * NB;
   static constexpr int kStage = kWarps * kLoads * 2 * L::GB;
   // resident CTAs wanted: registers for outputs and queries decide
   static constexpr int kRegs = NB * (HD / 16 * 6 + 16);
-  static constexpr int kCtas = kSplit && (kRegs > 80 || 3 * kStage > 108 * 1024) ? 1 : 2;
+  static constexpr int kCtas = kRegs > 80 || 3 * kStage > 108 * 1024 ? 1 : 2;
   static constexpr int kRoom = 224 * 1024 / kCtas - 3072, kFit = kRoom / kStage;
   static constexpr int kStages = kFit < 3 ? 3 : kFit > 6 ? 6 : kFit;
   static constexpr int kMost = 216 * 1024 / kStage, kDeep = kMost > 8 ? 8 : kMost < kStages ? kStages : kMost;  // where a CTA has an SM to itself
-  static_assert(!kSplit || kWarps * kRows * HD * 4 <= 3 * kStage, "the warps' outputs are joined in the ring");
+  static constexpr int kMostSmem = kDeep * kStage;
+  static_assert(kWarps * kRows * HD * 4 <= 3 * kStage, "the warps' outputs are joined in the ring");
   // Tiles of an item that are not worth sharing (joining parts takes a second kernel), and the least share of one that is shared.
   static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile;
   static constexpr int kRestart = 768 / kTile;  // what another item costs a CTA, in tiles
@@ -358,6 +359,27 @@ struct Rows {  // 8 * NB rows of queries
   float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = 1 / v_ref, which is finite
 };
 
+// The power of two that brings a row's largest value to [256, 512): f16 is exact for what is above 2^-22 of it.
+__device__ __forceinline__ float to_f16_range(float top) {
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);
+  return top > 0.f && top < INFINITY ? __uint_as_float((uint32_t)min(254 + 8 - e, 254) << 23) : 1.f;
+}
+// Where four columns of a part's row lie: rows next to one another where a thread has a whole one, columns next to one another else.
+template <class F>
+__device__ __forceinline__ float4* part_at(const Attn& a, size_t slot, int row, int col4) {
+  return reinterpret_cast<float4*>(a.part) + (F::kSplit ? (slot * F::kRows + row) * (F::HD / 4) + col4 : (slot * (F::HD / 4) + col4) * F::kRows + row);
+}
+template <bool F16>
+__device__ __forceinline__ float from_16(uint16_t w) {
+  return F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+}
+// Parts of an item that begins in this CTA and does not end there: its own, and one of each of the next ones until the item ends.
+__device__ __forceinline__ void mark_shared(const Attn& a, const Plan& plan, const Item& it) {
+  const uint32_t last = plan.cut == kPieces ? blockIdx.x + (uint32_t)(it.tiles - 1) / (uint32_t)plan.share
+                                            : (uint32_t)(it.unit + it.tiles - 1) / (uint32_t)plan.share;
+  a.head[blockIdx.x] = make_int4(it.b, it.mt, it.head, (int)(last - blockIdx.x) + 1);
+}
+
 template <int HD, int NB>
 struct RawRows {
   uint2 w[NB][HD / 16];  // the thread's row g of each eight
@@ -399,10 +421,7 @@ __device__ __forceinline__ void begin_rows(const Attn& a, const Item& it, int ro
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the power of two that brings the row's largest value to [256, 512): f16 is exact for what is above 2^-22 of it
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);
-      const bool fine = top > 0.f && top < INFINITY;
-      const float by = fine ? __uint_as_float((uint32_t)min(254 + 8 - e, 254) << 23) : 1.f;
+      const float by = to_f16_range(top);
       mult /= by;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
@@ -455,10 +474,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 mat
 
 // KG * 16 keys at positions key0.. against the warp's rows; group i of them lies at ring + i * 2 * GB.  `checked`: some row does not
 // see some key.
-template <int HD, bool F8, int NB, int KG, bool kRest>
+template <int HD, bool F8, int NB, int KG>
 __device__ __forceinline__ void take_keys(const char* ring, const float2* scales, int key0, bool checked, int window, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
   constexpr int kChains = NB == 1 ? 2 : 1;
+  constexpr bool kRest = !F8;  // probabilities have one
   const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   float s[KG][NB][4];  // keys g (0, 1) and g + 8 (2, 3), rows 2 j and 2 j + 1
   float2 scale[KG];    // of keys, of values
@@ -695,7 +715,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
 template <class F>
 __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(const Attn a) {
   constexpr int HD = F::HD, NB = F::NB;
-  constexpr bool F8 = F::F8, kSplit = F::kSplit;
+  constexpr bool F8 = F::F8;
   using L = Layout<HD, F8>;
   constexpr int kRows = F::kRows, kWarps = F::kWarps, kLoads = F::kLoads, kTile = F::kTile, kThreads = F::kThreads;
   extern __shared__ __align__(128) char ring[];
@@ -711,13 +731,12 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
     return;
   }
   const uint32_t ring_at = smem_u32(ring);
-  const int warp_rows = kSplit ? 0 : warp * 8 * NB;  // the warp's first row of a tile's
   RawRows<HD, NB> raw;
-  fetch_queries<HD, F8, NB>(a, it, it.mt * kRows + warp_rows, raw);
+  fetch_queries<HD, F8, NB>(a, it, it.mt * kRows, raw);
 
   Rows<HD, F8, NB> r;
   for (;;) {
-    const int rows0 = it.mt * kRows + warp_rows, tile0 = it.range.template t0<F>() + it.off;
+    const int rows0 = it.mt * kRows, tile0 = it.range.template t0<F>() + it.off;
     // copies of tile0 + i, i < count: kLoads groups of 16 keys of each by this warp.  Where they lie (in 16-byte pieces; all ones:
     // nowhere) and their scales, of the next 32 groups, are in its lanes.
     constexpr int kAhead = 32 / kLoads;  // tiles
@@ -792,28 +811,25 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
 #pragma unroll 1
     for (int i = 0; i < a.stages - 1; ++i) put_scales();
     begin_rows<HD, F8, NB>(a, it, rows0, raw, r);
-    // positions of the warp's first and last row
-    const bool any_row = kSplit || rows0 < it.s.n * a.group;
-    const bool all = kSplit && a.one_tile;
-    const int p_first = it.s.pos + (all ? 0 : a.by_group(rows0));
-    const int p_last = it.s.pos + (all ? it.s.n - 1 : min(it.s.n - 1, a.by_group(rows0 + 8 * NB - 1)));
+    // positions of the first and last row
+    const int p_first = it.s.pos + (a.one_tile ? 0 : a.by_group(rows0));
+    const int p_last = it.s.pos + (a.one_tile ? it.s.n - 1 : min(it.s.n - 1, a.by_group(rows0 + 8 * NB - 1)));
 #pragma unroll 1
     for (int i = 0; i < it.count; ++i) {
       if (a.stages == F::kStages) copy_wait<F::kStages - 2>();
       else copy_wait<F::kDeep - 2>();
-      if (kSplit) __syncwarp();
-      else __syncthreads();
+      __syncwarp();
       copy(i + a.stages - 1);
       put_scales();
       const char* at = ring + from_stage * F::kStage;
       constexpr int KG = F::kGroups;
       const int key_tile = (tile0 + i) * kTile;
 #pragma unroll 1
-      for (int w = kSplit ? warp * kLoads : 0; w < (kSplit ? (warp + 1) * kLoads : kWarps * kLoads); w += KG) {
+      for (int w = warp * kLoads; w < (warp + 1) * kLoads; w += KG) {
         const int key0 = key_tile + w * kGroup;
-        if (!any_row || key0 > p_last || (a.window && key0 + KG * kGroup - 1 <= p_first - a.window)) continue;
+        if (key0 > p_last || (a.window && key0 + KG * kGroup - 1 <= p_first - a.window)) continue;
         const bool checked = key0 + KG * kGroup - 1 > p_first || (a.window && key0 <= p_last - a.window);
-        take_keys<HD, F8, NB, KG, kSplit && !F8>(at + w * 2 * L::GB, &scales[from_stage][w], key0, checked, a.window, r);
+        take_keys<HD, F8, NB, KG>(at + w * 2 * L::GB, &scales[from_stage][w], key0, checked, a.window, r);
       }
       if (++from_stage == a.stages) from_stage = 0;
     }
@@ -822,7 +838,7 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
     // the item's end; the queries of the next one are fetched meanwhile
     const Item done = it;
     const bool another = next_item<F>(a, plan, it);
-    if (another) fetch_queries<HD, F8, NB>(a, it, it.mt * kRows + warp_rows, raw);
+    if (another) fetch_queries<HD, F8, NB>(a, it, it.mt * kRows, raw);
     // rows' sums over their threads, and over the warps where those took different keys
     const bool begins = done.off == 0, ends = done.off + done.count == done.tiles, complete = begins && ends;
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
@@ -836,114 +852,75 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
         r.l[n][h] += __shfl_xor_sync(0xffffffffu, r.l[n][h], 8);
         r.l[n][h] += __shfl_xor_sync(0xffffffffu, r.l[n][h], 16);
       }
-    if (kSplit) {
-      __syncthreads();  // all warps are done with the ring, which now takes their outputs
-      float* o_at = reinterpret_cast<float*>(ring);
+    __syncthreads();  // all warps are done with the ring, which now takes their outputs
+    float* o_at = reinterpret_cast<float*>(ring);
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = 8 * n + 2 * j + h;
-          if (g == 0) {
-            join_m[warp][row] = r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h];
-            join_l[warp][row] = r.l[n][h];
-          }
-#pragma unroll
-          for (int y = 0; y < HD / 16; ++y) {
-            float* at = o_at + (warp * kRows + row) * HD;
-            at[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
-            at[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
-          }
+      for (int h = 0; h < 2; ++h) {
+        const int row = 8 * n + 2 * j + h;
+        if (g == 0) {
+          join_m[warp][row] = r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h];
+          join_l[warp][row] = r.l[n][h];
         }
-      __syncthreads();
-      const int first = done.mt * kRows, n_rows = min(kRows, done.s.n * a.group - first);
-      for (int k = tid; k < n_rows * (HD / 4); k += kThreads) {
-        const int row = k / (HD / 4), col = k % (HD / 4) * 4;
-        float top = join_m[0][row];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w][row]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float by = exp2_fast(join_m[w][row] - base);
-          const float4 v = *reinterpret_cast<const float4*>(o_at + (w * kRows + row) * HD + col);
-          l += join_l[w][row] * by;
-          o[0] += v.x * by; o[1] += v.y * by; o[2] += v.z * by; o[3] += v.w * by;
-        }
-        if (complete) {
-          const float by = l == 0.f ? 0.f : 1.f / l;
-          const int t = a.by_group(first + row), hd = first + row - t * a.group;
-          *reinterpret_cast<uint2*>(a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD + col) =
-              make_uint2(pack<false>(o[0] * by, o[1] * by), pack<false>(o[2] * by, o[3] * by));
-        } else {
-          *reinterpret_cast<float4*>(a.part + ((size_t)slot * kRows + row) * HD + col) = make_float4(o[0], o[1], o[2], o[3]);
-          if (col == 0) a.stats[(size_t)slot * kRows + row] = make_float2(top, l);
+        for (int y = 0; y < HD / 16; ++y) {
+          float* at = o_at + (warp * kRows + row) * HD;
+          at[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
+          at[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
         }
       }
-    } else {
+    __syncthreads();
+    const int first = done.mt * kRows, n_rows = min(kRows, done.s.n * a.group - first);
+    for (int k = tid; k < n_rows * (HD / 4); k += kThreads) {
+      const int row = k / (HD / 4), col = k % (HD / 4) * 4;
+      float top = join_m[0][row];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int rows = done.s.n * a.group - done.mt * kRows;  // of the tile
-        if (complete) {
-          float by[2];
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w][row]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) by[h] = r.l[n][h] == 0.f ? 0.f : unit_o / r.l[n][h];
-          // transposed: columns 2 j and 2 j + 1 of a group of eight, or of pairs of them, for row g
-          const int row = warp_rows + 8 * n + g, at = done.mt * kRows + row, t = a.by_group(at), hd = at - t * a.group;
-          bf16* out = a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD;
-#pragma unroll
-          for (int y = 0; y < HD / 16; ++y) {
-            const uint32_t u = transposed(pack<false>(r.o[n][y][0] * by[0], r.o[n][y][1] * by[1]));
-            const uint32_t v = transposed(pack<false>(r.o[n][y][2] * by[0], r.o[n][y][3] * by[1]));
-            if (row >= rows) continue;
-            if (F8) {  // element 2 y and element 2 y + 1, neighbours, of threads 2 j and 2 j + 1
-              *reinterpret_cast<uint32_t*>(out + column<HD, F8>(2 * y, 2 * j)) = __byte_perm(u, v, 0x5410);
-              *reinterpret_cast<uint32_t*>(out + column<HD, F8>(2 * y, 2 * j + 1)) = __byte_perm(u, v, 0x7632);
-            } else {
-              *reinterpret_cast<uint32_t*>(out + 16 * y + 2 * j) = u;
-              *reinterpret_cast<uint32_t*>(out + 16 * y + 8 + 2 * j) = v;
-            }
-          }
-          continue;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = warp_rows + 8 * n + 2 * j + h;
-          if (row >= rows) continue;
-          float* part = a.part + ((size_t)slot * kRows + row) * HD;
-          if (g == 0) a.stats[(size_t)slot * kRows + row] = make_float2(r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h], r.l[n][h]);
-#pragma unroll
-          for (int y = 0; y < HD / 16; ++y) {
-            part[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
-            part[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
-          }
-        }
+      for (int w = 0; w < kWarps; ++w) {
+        const float by = exp2_fast(join_m[w][row] - base);
+        const float4 v = *reinterpret_cast<const float4*>(o_at + (w * kRows + row) * HD + col);
+        l += join_l[w][row] * by;
+        o[0] += v.x * by; o[1] += v.y * by; o[2] += v.z * by; o[3] += v.w * by;
+      }
+      if (complete) {
+        const float by = l == 0.f ? 0.f : 1.f / l;
+        const int t = a.by_group(first + row), hd = first + row - t * a.group;
+        *reinterpret_cast<uint2*>(a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD + col) =
+            make_uint2(pack<false>(o[0] * by, o[1] * by), pack<false>(o[2] * by, o[3] * by));
+      } else {
+        *part_at<F>(a, slot, row, col / 4) = make_float4(o[0], o[1], o[2], o[3]);
+        if (col == 0) a.stats[(size_t)slot * kRows + row] = make_float2(top, l);
       }
     }
-    if (!complete && begins && tid == 0) {
-      // parts: this CTA's and one of each of the next ones until the item ends
-      const uint32_t last = plan.cut == kPieces ? blockIdx.x + (uint32_t)(done.tiles - 1) / (uint32_t)plan.share
-                                                : (uint32_t)(done.unit + done.tiles - 1) / (uint32_t)plan.share;
-      a.head[blockIdx.x] = make_int4(done.b, done.mt, done.head, (int)(last - blockIdx.x) + 1);
-    }
+    if (!complete && begins && tid == 0) mark_shared(a, plan, done);
     if (!another) break;
     __syncthreads();  // the ring and the join buffers are free again
   }
   pdl_trigger();  // not earlier: the next kernel's CTAs would take the room of this one's second half
 }
 
+}  // namespace
+}  // namespace ane
+#include "kv_attention_tc.cuh"
+namespace ane {
+namespace {
+
 // Joins the parts of shared items: a block for each CTA of the first kernel and row of a tile.  Factors of all parts first, so that the
 // parts themselves are read without waiting for one another.
 constexpr int kJoinThreads = 256, kMostParts = 1024;
 
-template <int HD, int kRows>
+template <class F>
 __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int row) {
+  constexpr int HD = F::HD, kRows = F::kRows;
   const Span s = span_of(a.batch, item.x, INT32_MAX, INT32_MAX, a.status);
   const int at = item.y * kRows + row, parts = item.w, tid = threadIdx.x, warp = tid >> 5;
   if (at >= s.n * a.group) return;
   // part i: the first CTA's second slot, then the first slot of each
-  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row; };
+  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)); };
   constexpr int lanes = HD / 4, teams = kJoinThreads / lanes, kMine = kMostParts / kJoinThreads;  // a team takes every teams-th part
   __shared__ float factor[kMostParts];
   __shared__ float most[kJoinThreads / 32], total[kJoinThreads / 32];
@@ -954,14 +931,14 @@ __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int 
 #pragma unroll
   for (int k = 0; k < kMine; ++k) {
     const int i = tid + k * kJoinThreads;
-    st[k] = i < parts ? a.stats[slot(i)] : make_float2(-INFINITY, 0.f);
+    st[k] = i < parts ? a.stats[slot(i) * kRows + row] : make_float2(-INFINITY, 0.f);
   }
   constexpr int kEarly = 8;  // parts that are on their way before the factors are known
   float4 early[kEarly];
 #pragma unroll
   for (int k = 0; k < kEarly; ++k) {
     const int i = team + k * teams;
-    early[k] = team < teams && i < parts ? *reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    early[k] = team < teams && i < parts ? *part_at<F>(a, slot(i), row, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 #pragma unroll
   for (int k = 0; k < kMine; ++k) m = fmaxf(m, st[k].x);
@@ -992,7 +969,7 @@ __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int 
       if (team + k * teams < parts) add(early[k], factor[team + k * teams]);
 #pragma unroll 4
     for (int i = team + kEarly * teams; i < parts; i += teams)
-      add(*reinterpret_cast<const float4*>(a.part + slot(i) * HD + lane * 4), factor[i]);
+      add(*part_at<F>(a, slot(i), row, lane), factor[i]);
     sums[team][lane] = o;
   }
   __syncthreads();
@@ -1014,21 +991,22 @@ __device__ __forceinline__ void join_row(const Attn& a, int cta, int4 item, int 
 // The same of eight rows from `row` on by a block, for at most kFew parts: a row takes as many lanes as it has groups of four columns, rounded up to
 // a power of two.
 constexpr int kFew = 6;
-template <int HD, int kRows>
+template <class F>
 __device__ __forceinline__ void join_rows(const Attn& a, int cta, int4 item, int row0) {
-  constexpr int lanes = HD <= 32 ? 8 : HD <= 64 ? 16 : 32;
+  constexpr int HD = F::HD, kRows = F::kRows, lanes = HD <= 32 ? 8 : HD <= 64 ? 16 : 32;
   const Span s = span_of(a.batch, item.x, INT32_MAX, INT32_MAX, a.status);
-  const int parts = item.w, lane = threadIdx.x % lanes, row = row0 + threadIdx.x / lanes, at = item.y * kRows + row;
-  if (threadIdx.x / lanes >= 8 || row >= kRows || at >= s.n * a.group) return;
+  const int tid = threadIdx.x, parts = item.w, lane = F::kSplit ? tid % lanes : tid / 8, row = row0 + (F::kSplit ? tid / lanes : tid % 8);
+  const int at = item.y * kRows + row;
+  if (tid >= 8 * lanes || row >= kRows || at >= s.n * a.group) return;
   const bool mine = lane * 4 < HD;
   float2 st[kFew];
   float4 v[kFew];
 #pragma unroll
   for (int i = 0; i < kFew; ++i) {
     // part i: the first CTA's second slot, then the first slot of each
-    const size_t slot = (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kRows + row;
-    st[i] = i < parts ? a.stats[slot] : make_float2(-INFINITY, 0.f);
-    v[i] = i < parts && mine ? *reinterpret_cast<const float4*>(a.part + slot * HD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const size_t slot = (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i));
+    st[i] = i < parts ? a.stats[slot * kRows + row] : make_float2(-INFINITY, 0.f);
+    v[i] = i < parts && mine ? *part_at<F>(a, slot, row, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -1051,7 +1029,7 @@ __device__ __forceinline__ void join_rows(const Attn& a, int cta, int4 item, int
 // Rows of shared items, task t: row t % rows of the item that begins in CTA t / rows.  Most CTAs of the first kernel begin none: 32 tasks are
 // looked at together.  Items of up to kFew parts take a part of a block a row, eight rows from every eighth task, others a block.
 // The grid's size is odd where a block has several tasks, so that those are spread evenly.
-template <int HD, int kRows>
+template <class F>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int ctas, int rows) {
   pdl_trigger();
   pdl_wait();
@@ -1064,10 +1042,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int
       const int4 one = make_int4(__shfl_sync(0xffffffffu, item.x, from), __shfl_sync(0xffffffffu, item.y, from),
                                  __shfl_sync(0xffffffffu, item.z, from), __shfl_sync(0xffffffffu, item.w, from));
       if (one.w <= kFew) {
-        join_rows<HD, kRows>(a, cta, one, row);
+        join_rows<F>(a, cta, one, row);
         continue;
       }
-      join_row<HD, kRows>(a, cta, one, row);
+      join_row<F>(a, cta, one, row);
       __syncthreads();
     }
   }
@@ -1076,10 +1054,13 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const Attn a, int
 template <class F>
 cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
   constexpr int kRows = F::kRows, kTile = F::kTile, most = F::kCtas;
-  static_assert(most <= 2 && kRows <= (F::HD <= 64 ? 128 : 64), "the workspace is sized for these");
+  static_assert(most * kRows <= (F::HD <= 64 ? 256 : 128), "the workspace is sized for these");
   static unsigned long long opted = 0;
-  auto kernel = kv_attention_kernel<F>;
-  if (!smem_opt_in(kernel, F::kDeep * F::kStage, opted)) return cudaGetLastError();
+  auto kernel = [] {
+    if constexpr (F::kSplit) return kv_attention_kernel<F>;
+    else return kv_prompt_kernel<F>;
+  }();
+  if (!smem_opt_in(kernel, F::kMostSmem, opted)) return cudaGetLastError();
   a.one_tile = (long long)a.max_new * a.group <= kRows;
   // no more CTAs than there can be units: items, or shares of F::kLeast tiles of them
   const long long longest = a.window ? min((long long)a.capacity, (long long)a.window + (kRows - 1) / a.group + kTile) : a.capacity;
@@ -1096,24 +1077,26 @@ cudaError_t run(Attn a, int sms, void* workspace, cudaStream_t s) {
   a.stats = reinterpret_cast<float2*>(at);
   at += sizeof(float2) * 2 * (size_t)sms * most * kRows;
   a.part = reinterpret_cast<float*>(at);
-  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(F::kThreads), a.stages * F::kStage, s, a);
+  cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(F::kThreads), F::kSplit ? a.stages * F::kStage : F::kMostSmem, s, a);
   if (e != cudaSuccess || !may_share) return e;
   const int rows = (int)min((long long)kRows, (long long)a.max_new * a.group);
-  return launch_pdl(kv_join_kernel<F::HD, kRows>, dim3((unsigned)min((long long)ctas * rows, (kRows > 32 ? 8ll : 4ll) * sms - 1)), dim3(kJoinThreads), 0, s, a, ctas, rows);
+  return launch_pdl(kv_join_kernel<F>, dim3((unsigned)min((long long)ctas * rows, (kRows > 32 ? 8ll : 4ll) * sms - 1)), dim3(kJoinThreads), 0, s, a, ctas, rows);
 }
 
-// Which form, by the rows of one KV head that a sequence has at most.  Tiles of few rows that all warps share leave no warp without rows and
-// are read again for the next tile; tiles of many rows are read once.  Two sequences of 60000 tokens: 32 rows of 128 36 us by the
-// first, 46 by the second, 48 rows 47 and 48, 64 rows 57 and 56 (bf16 54 and 41); 60 rows of 64 65 and 70 (bf16 60 and 57), 96 rows 85 and 74;
-// 16 sequences of 500 tokens, 60 rows of 64 13.6 and 22.4, 120 rows 24.0 and 23.2.
+// Which form, by the rows of one KV head that a sequence has at most.  Up to 32 the warps share them: as one tile, or, of wide heads, whose outputs
+// do not fit the registers otherwise, two tiles that read their keys again; more are products of 128 rows.  us, the first and the second:
+//   two sequences of 60000 tokens   20 rows of 64 81 and 94, 32 83 and 95, 48 142 and 98, 64 142 and 102 (bf16 136 and 89);
+//                                   32 rows of 128 36 and 40 (bf16 35 and 34)
+//   64 sequences of 8192            32 rows of 64 290 and 292, 64 474 and 301; 24 rows of 128 83 and 99, 32 88 and 100
+//   16 sequences of 500             20 rows of 48 11.6 and 12.7, 48 12.2 and 12.9, 64 21.0 and 13.4
 template <int HD, bool F8>
 cudaError_t run_rows(const Attn& a, int sms, void* workspace, cudaStream_t s) {
   const long long rows = (long long)a.max_new * a.group;
-  if (rows <= 8) return run<Form<HD, F8, 1, true>>(a, sms, workspace, s);
-  if (rows <= (HD <= 64 ? 16 : 32)) return run<Form<HD, F8, 2, true>>(a, sms, workspace, s);
+  if (rows <= 8) return run<Form<HD, F8, 1>>(a, sms, workspace, s);
+  if (rows <= (HD <= 64 ? 16 : 32)) return run<Form<HD, F8, 2>>(a, sms, workspace, s);
   if constexpr (HD <= 64)
-    if (rows <= 64) return run<Form<HD, F8, 4, true>>(a, sms, workspace, s);
-  return run<Form<HD, F8, HD <= 64 ? 4 : 2, false>>(a, sms, workspace, s);
+    if (rows <= 32) return run<Form<HD, F8, 4>>(a, sms, workspace, s);
+  return run<Prompt<HD, F8>>(a, sms, workspace, s);
 }
 template <int HD>
 cudaError_t run_hd(const Attn& a, int sms, void* workspace, cudaStream_t s) {
@@ -1129,7 +1112,7 @@ static size_t workspace_of(int sms) {
   auto bytes = [&](size_t per_sm, size_t rows) {
     return sms * per_sm * (sizeof(int4) + 2 * rows * (sizeof(float2) + sizeof(float) * HD));
   };
-  return bytes(2, HD <= 64 ? 128 : 64);  // the form of most rows, and no form has more CTAs
+  return bytes(HD <= 64 ? 2 : 1, 128);  // the form of most rows
 }
 size_t kv_attention_workspace(int sms, int hd) {  // the same for both types of cache
   switch (hd) {

@@ -379,6 +379,63 @@ def test_attention_visible_nan_reaches_its_row_only(kind, new):
     assert nan[-1, :, 0].all() and nan.sum() == heads
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd,page", [(8, 1, 32, 16), (6, 6, 48, 48), (12, 4, 64, 64), (12, 4, 96, 16), (16, 2, 128, 32)])
+@pytest.mark.parametrize("window", [0, 130])
+def test_attention_of_prompts(kind, heads, kv, hd, page, window):
+    # tiles of rows that end inside a sequence, keys from none before to many, prompts beside single tokens
+    check_attention(kind, heads, kv, hd, page, [150, 33, 1, 0, 260], [700, 0, 64, 9, 5], window=window)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 1, 32), (4, 2, 96), (8, 1, 128)])
+def test_attention_of_prompts_in_many_shared_parts(kind, heads, kv, hd):
+    check_attention(kind, heads, kv, hd, 64, [70, 9], [20001, 300])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("pos,at", [(0, 40), (0, 99), (300, 350)])
+def test_attention_of_prompts_nan_reaches_later_rows_only(kind, hd, pos, at):
+    """A value that is NaN, of a token of the prompt: rows before it are what they are without it, its own and later ones have a NaN in its column."""
+    heads, kv, page, new = 6, 2, 64, 100
+    cache, q, want = check_attention(kind, heads, kv, hd, page, [new], [pos], hidden_nan=False)
+    es, column = (2, hd - 1) if kind == "bf16" else (1, hd - 1)
+    first = (at % page) * hd * es + column * es  # of KV head 0
+    cache.v.view(torch.uint8)[cache.table_host[0][at // page], first:first + es] = torch.tensor([0xc0, 0x7f][-es:], dtype=torch.uint8, device="cuda")
+    out = torch.full_like(want, 7.0)
+    attention(cache, heads, q, out, i32([0, new]), i32([pos]), new)
+    assert status() == 0
+    nan = torch.isnan(out.float()).view(new, heads, hd).cpu()
+    assert nan[at - pos:, :heads // kv, column].all() and int(nan.sum()) == (new - (at - pos)) * (heads // kv)
+    # the tile's products are summed one by one instead: rounding of probabilities is the same, the order of sums is not
+    k, v = cache.rows("k", 0, pos + new), cache.rows("v", 0, pos + new)
+    v[at] = 0
+    mq = q.double().cpu().view(new, heads, hd)
+    ref, mass, big = attention_exact(mq, k, v, pos, hd ** -0.5, 0)
+    tol = attention_tolerance(ref, mass, big, kind, hd, pos + new, mq, hd ** -0.5, float(k.abs().max()))
+    before = slice(0, at - pos)
+    assert ((out.double().cpu().view(new, heads, hd) - ref).abs() <= tol)[before].all()
+
+
+def test_prompts_of_two_head_sizes_on_two_streams():
+    sizes = [(4, 1, 64, "bf16"), (4, 1, 128, "e4m3")]
+    caches = [Cache([2100, 700], kv, hd, 64, kind, seed=i) for i, (_, kv, hd, kind) in enumerate(sizes)]
+    q = [torch.randn(200, h * hd, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).cuda() for i, (h, _, hd, _) in enumerate(sizes)]
+    start, pos = i32([0, 100, 200]), i32([2000, 600])
+    want = [torch.empty_like(x) for x in q]
+    for i, (h, _, _, _) in enumerate(sizes):
+        attention(caches[i], h, q[i], want[i], start, pos, 100)
+    works, streams = [workspace(h, kv, hd) for h, kv, hd, _ in sizes], [torch.cuda.Stream() for _ in sizes]
+    got = [[torch.empty_like(x) for _ in range(20)] for x in q]
+    torch.cuda.synchronize()
+    for k in range(20):
+        for i, (h, _, _, _) in enumerate(sizes):
+            attention(caches[i], h, q[i], got[i][k], start, pos, 100, work=works[i], stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    assert status() == 0 and all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
 def test_attention_offsets_beyond_32_bits():
     # pages 2^28 bytes apart: the last ones begin behind 2^32
     kv, hd, page, pages, stride = 1, 64, 16, 20, 1 << 28
