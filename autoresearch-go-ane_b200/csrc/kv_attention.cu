@@ -28,7 +28,7 @@ constexpr int kGroup = 16;  // keys of a product
 // A row's maximum follows its scores only where they exceed it by more than this (in log2), so that probabilities are below 2^kSlack: most
 // keys then need no exchange of maxima and no new factor on what has been summed.
 constexpr float kSlack = 8.f;
-constexpr float kPScale = 128.f;  // of f16 probabilities, 2^15 at most then: those down to 2^-21 of the maximum's stay normal
+constexpr float kPScale = 128.f;  // of f16 probabilities, 2^15 at most then: those down to 2^-21 of the maximum's stay normal, below 2^-32 they are 0
 constexpr float kLowest = 1.17549435e-38f;
 
 struct Attn {
@@ -72,7 +72,7 @@ struct Form {
   // resident CTAs wanted: registers for outputs and queries decide
   static constexpr int kRegs = NB * (HD / 16 * 6 + 16);
   static constexpr int kCtas = kRegs > 80 || 3 * kStage > 108 * 1024 ? 1 : 2;
-  static constexpr int kRoom = 224 * 1024 / kCtas - 3072, kFit = kRoom / kStage;
+  static constexpr int kRoom = 224 * 1024 / kCtas - 3 * 1024, kFit = kRoom / kStage;
   static constexpr int kStages = kFit < 3 ? 3 : kFit > 6 ? 6 : kFit;
   static constexpr int kMost = 216 * 1024 / kStage, kDeep = kMost > 8 ? 8 : kMost < kStages ? kStages : kMost;  // where a CTA has an SM to itself
   static constexpr int kMostSmem = kDeep * kStage;
