@@ -15,6 +15,10 @@
 // Work is cut on the device, as only the device knows the lengths: all tiles of keys of all (sequence, row tile, KV head) in one
 // line, an even share of the line to each CTA of one wave.  What a CTA did of an item that others share goes to the
 // workspace, and a second kernel joins the parts in their order, without atomics: the same sums from call to call.
+//
+// Single tokens, 32 heads of 128 with 8 for keys, 64 sequences of up to 8000 tokens: 208 us from bf16 pages (6.5 TB/s, the memory's rate), 118 to
+// 128 from 8-bit ones (5.3 to 5.7 TB/s; the floor is 103), where instructions that widen, scale and exponentiate bound it.  Small calls are
+// launches and dependent reads: one sequence of 256 tokens 5.7 us, 32 of 768 8.9, two of 60000 with two KV heads 19.8 (the floor is 7.3).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

@@ -12,8 +12,9 @@
 // The 8192 exponentials of a tile take 512 cycles of an SM at 16 a cycle; the products 256 with heads of 64.  Heads of up to 64 have two CTAs an
 // SM, so that one's waits and copies run under the other's softmax: 850 to 1000 cycles a tile and SM.  Eight sequences of 400 tokens over 1500,
 // 12 heads of 64 with 4 for keys: 49 us from 8-bit pages and 41 from bf16 (8.2 GFLOP; by mma.sync, every warp converting all keys, 74 and 59),
-// of which 4 go into cutting the work and 8 into joining shared items; two of 100 over 60000, 16 heads of 128 with 2, 157 and 126 (334 by
-// mma.sync).  Two threads a row, with half of the keys each, took 60 and 49 in place of 52 and 45: registers for 22 warps are too few.
+// of which 4 go into cutting the work and 8 into joining shared items; two of 100 over 60000, 16 heads of 128 with 2, 161 and 127 (334 by
+// mma.sync).  Two threads a row, with half of the keys each, took 60 and 49 in place of 52 and 45: registers for 22 warps are too few; half of the
+// scores loaded under the maximum of the others 50.4 and 42.6 in place of 49.2 and 41.6.
 // Every wait is bounded and reports through the status word.
 #pragma once
 
