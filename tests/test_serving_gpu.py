@@ -418,6 +418,27 @@ def test_attention_of_prompts_nan_reaches_later_rows_only(kind, hd, pos, at):
     assert ((out.double().cpu().view(new, heads, hd) - ref).abs() <= tol)[before].all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_captured_prompt_replayed_at_other_places(kind):
+    heads, kv, hd, new = 8, 2, 64, 90
+    cache = Cache([700], kv, hd, 64, kind, seed=6)
+    q = torch.randn(new, heads * hd, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).cuda()
+    want, out, work = torch.empty_like(q), torch.empty_like(q), workspace(heads, kv, hd)
+    start, pos, stream = i32([0, new]), i32([0]), torch.cuda.Stream()
+    attention(cache, heads, q, want, start, pos, new, work=work)  # and everything that a first call does
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        attention(cache, heads, q, out, start, pos, new, work=work, stream=stream.cuda_stream)
+    for at in (0, 37, 610):
+        pos.fill_(at)
+        attention(cache, heads, q, want, start, pos, new, work=work)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert status() == 0 and torch.equal(out, want)
+
+
 def test_prompts_of_two_head_sizes_on_two_streams():
     sizes = [(4, 1, 64, "bf16"), (4, 1, 128, "e4m3")]
     caches = [Cache([2100, 700], kv, hd, 64, kind, seed=i) for i, (_, kv, hd, kind) in enumerate(sizes)]
