@@ -32,8 +32,21 @@ constexpr int kGroup = 16;  // keys of a product
 // A row's maximum follows its scores only where they exceed it by more than this (in log2), so that probabilities are below 2^kSlack: most
 // keys then need no exchange of maxima and no new factor on what has been summed.
 constexpr float kSlack = 8.f;
-constexpr float kPScale = 128.f;  // of f16 probabilities, 2^15 at most then: those down to 2^-21 of the maximum's stay normal, below 2^-32 they are 0
 constexpr float kLowest = 1.17549435e-38f;
+
+// What enters the products with 8-bit values is a probability times its page's scale, in f16.  Scales of the pages that a row sees may be of any
+// sizes, so the unit follows the row's own largest such product w, as the exponents' base follows its largest score: outputs are in units of
+// 2^(w - 7), f16 numbers 2^15 at most; those down to 2^-21 of the largest stay normal, below 2^-32 they are 0.  What a row does not see has no part
+// in it.  With f = 2^((base - w + 7) / 2) a probability takes the factor scale * f * f, in two steps as base - w may be 134; where it leaves fp32,
+// above 2^127, the page is one that the row does not see, or whose probabilities are below 2^-112.
+constexpr float kNoUnit = -3e38f;  // log2 of the largest product of a row that has seen none
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float unit_factor(float base, float w) { return exp2_fast(fminf(0.5f * (base - w) + 3.5f, 72.f)); }
+__device__ __forceinline__ float into_units(float scale, float f) { return fminf(scale * f * f, 0x1p127f); }
 
 struct Attn {
   PagedKv kv;
@@ -137,11 +150,6 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   uint32_t r;
   if (F8) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ void copy_16(uint32_t dst, const void* src, bool take) {
@@ -360,7 +368,7 @@ struct Rows {  // 8 * NB rows of queries
   // and what brings products to scores in log2
   float base[NB][2], limit[NB][2], l[NB][2], mult[NB][2];
   int pos[NB][2];                         // their positions; -1: no such row
-  float v_ref, v_inv;                     // 8 bits: o is in units of v_ref / kPScale; v_inv = 1 / v_ref, which is finite
+  float w[NB][2], f[NB][2];               // 8 bits: log2 of the largest probability times scale, and what makes f16 numbers of such products
 };
 
 // The power of two that brings a row's largest value to [256, 512): f16 is exact for what is above 2^-22 of it.
@@ -447,13 +455,15 @@ __device__ __forceinline__ void begin_rows(const Attn& a, const Item& it, int ro
       r.base[n][h] = 0.f;
       r.limit[n][h] = -INFINITY;
       r.l[n][h] = 0.f;
+      if (F8) {
+        r.w[n][h] = kNoUnit;
+        r.f[n][h] = unit_factor(0.f, kNoUnit);
+      }
       r.mult[n][h] = F8 ? __shfl_sync(0xffffffffu, mult, (2 * j + h) * 4) : mult;
     }
 #pragma unroll
     for (int y = 0; y < HD / 16; ++y) r.o[n][y][0] = r.o[n][y][1] = r.o[n][y][2] = r.o[n][y][3] = 0.f;
   }
-  r.v_ref = kLowest;
-  r.v_inv = 1.f / kLowest;
 }
 
 // Whether one of a word's values is infinite or NaN.
@@ -479,17 +489,17 @@ __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 mat
 // KG * 16 keys at positions key0.. against the warp's rows; group i of them lies at ring + i * 2 * GB.  `checked`: some row does not
 // see some key.
 template <int HD, bool F8, int NB, int KG>
-__device__ __forceinline__ void take_keys(const char* ring, const float2* scales, int key0, bool checked, int window, Rows<HD, F8, NB>& r) {
+__device__ __forceinline__ void take_keys(const char* ring, const float4* scales, int key0, bool checked, int window, Rows<HD, F8, NB>& r) {
   using L = Layout<HD, F8>;
   constexpr int kChains = NB == 1 ? 2 : 1;
   constexpr bool kRest = !F8;  // probabilities have one
   const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   float s[KG][NB][4];  // keys g (0, 1) and g + 8 (2, 3), rows 2 j and 2 j + 1
-  float2 scale[KG];    // of keys, of values
+  float4 scale[KG];    // of keys, of values, log2 of the latter
 #pragma unroll
   for (int k = 0; k < KG; ++k) {
     const char* ks = ring + k * 2 * L::GB;
-    scale[k] = F8 ? scales[k] : make_float2(1.f, 1.f);
+    scale[k] = F8 ? scales[k] : make_float4(1.f, 1.f, 0.f, 0.f);
     float even[NB][4];  // a second chain of products, half as long each
     auto products = [&](const uint32_t (&a)[4], int step) {
 #pragma unroll
@@ -541,25 +551,6 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
           if (key > pos || (window && key <= pos - window)) s[k][n][i] = -INFINITY;
         }
   }
-  float into[KG];
-  if (F8) {
-    float most = scale[0].y;
-#pragma unroll
-    for (int k = 1; k < KG; ++k) most = fmaxf(most, scale[k].y);
-    if (most > r.v_ref) {  // statistics keep their unit, the output changes to the new one
-      const float by = r.v_ref / most;
-      r.v_ref = most;
-      r.v_inv = 1.f / most;
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int y = 0; y < HD / 16; ++y)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r.o[n][y][i] *= by;
-    }
-#pragma unroll
-    for (int k = 0; k < KG; ++k) into[k] = scale[k].y * r.v_inv * kPScale;
-  }
   uint32_t p[KG][NB][2], rest[kRest ? KG : 1][NB][2];
   bool above = false;
   float mult[KG][NB][2];
@@ -567,13 +558,15 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float top = -INFINITY;
+      float top = -INFINITY, most = -INFINITY;
 #pragma unroll
       for (int k = 0; k < KG; ++k) {
         mult[k][n][h] = F8 ? fmaxf(r.mult[n][h] * scale[k].x, kLowest) : r.mult[n][h];  // not 0, so that hidden scores stay -infinity
-        top = fmaxf(top, fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h]);
+        const float high = fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h];
+        top = fmaxf(top, high);
+        if (F8) most = fmaxf(most, high + scale[k].z);
       }
-      above |= top > r.limit[n][h];
+      above |= top > r.limit[n][h] || (F8 && most > r.w[n][h] + kSlack);
     }
   if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -581,18 +574,30 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
       float fix[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float top = -INFINITY;
+        float top = -INFINITY, most = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < KG; ++k) top = fmaxf(top, fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        for (int k = 0; k < KG; ++k) {
+          const float high = fmaxf(s[k][n][h], s[k][n][2 + h]) * mult[k][n][h];
+          top = fmaxf(top, high);
+          if (F8) most = fmaxf(most, high + scale[k].z);
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (F8) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
         const bool none = r.limit[n][h] == -INFINITY;
         const float base = none ? (top == -INFINITY ? 0.f : top) : fmaxf(top, r.base[n][h]);
         fix[h] = none ? 1.f : exp2_fast(r.base[n][h] - base);  // sums are still 0 then
         r.base[n][h] = base;
         r.limit[n][h] = none && top == -INFINITY ? -INFINITY : base + kSlack;
         r.l[n][h] *= fix[h];
+        if (F8) {
+          const float w = fmaxf(most, r.w[n][h]);
+          fix[h] = exp2_fast(r.w[n][h] - w);
+          r.w[n][h] = w;
+          r.f[n][h] = unit_factor(base, w);
+        }
       }
 #pragma unroll
       for (int y = 0; y < HD / 16; ++y)
@@ -618,8 +623,9 @@ __device__ __forceinline__ void take_keys(const char* ring, const float2* scales
 #pragma unroll
     for (int k = 0; k < KG; ++k) {
       if (F8) {
+        const float into[2] = {into_units(scale[k].y, r.f[n][0]), into_units(scale[k].y, r.f[n][1])};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[k][n][i] *= into[k];
+        for (int i = 0; i < 4; ++i) s[k][n][i] *= into[i & 1];
       }
       p[k][n][0] = transposed(pack<F8>(s[k][n][0], s[k][n][1]));
       p[k][n][1] = transposed(pack<F8>(s[k][n][2], s[k][n][3]));
@@ -723,7 +729,7 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
   using L = Layout<HD, F8>;
   constexpr int kRows = F::kRows, kWarps = F::kWarps, kLoads = F::kLoads, kTile = F::kTile, kThreads = F::kThreads;
   extern __shared__ __align__(128) char ring[];
-  __shared__ float2 scales[F::kDeep][kWarps * kLoads];
+  __shared__ float4 scales[F::kDeep][kWarps * kLoads];
   __shared__ float join_m[kWarps][8 * NB], join_l[kWarps][8 * NB];
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
@@ -805,7 +811,7 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
     int scaled = 0, scale_stage = 0;
     auto put_scales = [&]() {
       if (F8 && scaled < it.count) {
-        if (lane / kLoads == scaled % kAhead) scales[scale_stage][warp * kLoads + lane % kLoads] = make_float2(my_k, my_v);
+        if (lane / kLoads == scaled % kAhead) scales[scale_stage][warp * kLoads + lane % kLoads] = make_float4(my_k, my_v, __log2f(my_v), 0.f);
         ++scaled;
         if (++scale_stage == a.stages) scale_stage = 0;
       }
@@ -846,8 +852,6 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
     // rows' sums over their threads, and over the warps where those took different keys
     const bool begins = done.off == 0, ends = done.off + done.count == done.tiles, complete = begins && ends;
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
-    float unit_o = 1.f;
-    if (F8) unit_o = r.v_ref * (1.f / kPScale);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -863,6 +867,7 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 8 * n + 2 * j + h;
+        const float unit = F8 ? 1.f / r.f[n][h] : 1.f;
         if (g == 0) {
           join_m[warp][row] = r.limit[n][h] == -INFINITY ? -INFINITY : r.base[n][h];
           join_l[warp][row] = r.l[n][h];
@@ -870,8 +875,8 @@ __global__ void __launch_bounds__(F::kThreads, F::kCtas) kv_attention_kernel(con
 #pragma unroll
         for (int y = 0; y < HD / 16; ++y) {
           float* at = o_at + (warp * kRows + row) * HD;
-          at[column<HD, F8>(2 * y, g)] = r.o[n][y][h] * unit_o;
-          at[column<HD, F8>(2 * y + 1, g)] = r.o[n][y][2 + h] * unit_o;
+          at[column<HD, F8>(2 * y, g)] = F8 ? r.o[n][y][h] * unit * unit : r.o[n][y][h];
+          at[column<HD, F8>(2 * y + 1, g)] = F8 ? r.o[n][y][2 + h] * unit * unit : r.o[n][y][2 + h];
         }
       }
     __syncthreads();

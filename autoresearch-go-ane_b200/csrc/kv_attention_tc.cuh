@@ -127,7 +127,7 @@ __device__ __forceinline__ int swizzled(int row, int c, int atom) { return (c >>
 template <class F>
 struct PromptMemory {
   uint64_t full[F::kStages], empty[F::kStages], scores[2], outputs[2], probs[2], queries;
-  float2 scales[F::kInfo][4];      // of a tile's groups of 16 keys
+  float4 scales[F::kInfo][4];      // of a tile's groups of 16 keys: of keys, of values, log2 of the latter
   alignas(4) unsigned char odd[F::kInfo][4];  // not 0: a value is infinite or NaN and hidden from some row
   uint32_t tmem;
 };
@@ -267,7 +267,7 @@ __device__ __forceinline__ void prompt_load(const Attn& a, const Plan& plan, Ite
         }
       }
       copy_commit();
-      if (F::F8 && lane / F::kEach == i % kAhead) m.scales[n % F::kInfo][group0 + lane % F::kEach] = make_float2(my_k, my_v);
+      if (F::F8 && lane / F::kEach == i % kAhead) m.scales[n % F::kInfo][group0 + lane % F::kEach] = make_float4(my_k, my_v, __log2f(my_v), 0.f);
       ++issued;
       const int first = (tile0 + i) * F::kTile;
       edges = edges << 1 | (first + F::kTile - 1 > p_first || (a.window && first <= p_last - a.window) ? 1u : 0u);
@@ -367,7 +367,7 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
     const int rows0 = it.mt * F::kRows + warp * 32, n_rows = it.s.n * a.group, tile0 = it.range.template t0<F>() + it.off;
     const int pos = it.mt * F::kRows + row < n_rows ? it.s.pos + a.by_group(it.mt * F::kRows + row) : -1;
     const int p_first = it.s.pos + a.by_group(rows0), p_last = it.s.pos + min(it.s.n - 1, a.by_group(rows0 + 31));
-    float base = 0.f, limit = -INFINITY, l = 0.f, v_ref = kLowest, v_inv = 1.f / kLowest;
+    float base = 0.f, limit = -INFINITY, l = 0.f, w = kNoUnit, f = unit_factor(0.f, kNoUnit);
 #pragma unroll 1
     for (int i = 0; i < it.count; ++i, ++n) {
       const int key0 = (tile0 + i) * kTile;
@@ -384,33 +384,34 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
         for (int e = 0; e < kTile; ++e)
           if (key0 + e > pos || (a.window && key0 + e <= pos - a.window)) s[e] = -INFINITY;
       }
-      float mults[4], into[4], most = 0.f, top = -INFINITY;
+      float mults[4], into[4], most = -INFINITY, top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        mults[g] = mult;
-        into[g] = 1.f;
-        if (F::F8) {
-          const float2 scale = m.scales[n % F::kInfo][g];
-          mults[g] = fmaxf(mult * scale.x, kLowest);  // not 0, so that hidden scores stay -infinity
-          into[g] = scale.y;
-          most = fmaxf(most, scale.y);
-        }
         float high = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) high = fmaxf(high, s[16 * g + e]);
+        mults[g] = mult;
+        into[g] = 1.f;
+        if (F::F8) {
+          const float4 scale = m.scales[n % F::kInfo][g];
+          mults[g] = fmaxf(mult * scale.x, kLowest);  // not 0, so that hidden scores stay -infinity
+          into[g] = scale.y;
+          most = fmaxf(most, fmaf(high, mults[g], scale.z));
+        }
         top = fmaxf(top, high * mults[g]);
       }
-      if (__any_sync(0xffffffffu, top > limit) || (F::F8 && most > v_ref)) {
+      if (__any_sync(0xffffffffu, top > limit || (F::F8 && most > w + kSlack))) {
         const bool none = limit == -INFINITY;
         const float up = top > limit ? (none ? (top == -INFINITY ? 0.f : top) : fmaxf(top, base)) : base;
         float fix = none ? 1.f : exp2_fast(base - up);  // the sum is still 0 then
         base = up;
         limit = none && top == -INFINITY ? -INFINITY : base + kSlack;
         l *= fix;
-        if (F::F8 && most > v_ref) {  // statistics keep their unit, the outputs change to the new one
-          fix *= v_ref / most;
-          v_ref = most;
-          v_inv = 1.f / most;
+        if (F::F8) {  // outputs have a unit of their own
+          const float now = most > w + kSlack ? most : w;
+          fix = exp2_fast(w - now);
+          w = now;
+          f = unit_factor(base, w);
         }
         if (i > 0) {
           if (!warp_wait(m.outputs[(n - 1) & 1], (n - 1) >> 1 & 1, a.status, DEV_MBAR_TIMEOUT_EPILOGUE)) return;
@@ -433,7 +434,7 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const uint64_t by = both(mults[g], mults[g]);
-        if (F::F8) into[g] = into[g] * v_inv * kPScale;  // in this order: v_inv may be 2^126
+        if (F::F8) into[g] = into_units(into[g], f);
 #pragma unroll
         for (int e = 8 * g; e < 8 * g + 8; ++e) {
           float lo, hi;
@@ -502,7 +503,7 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0), of = done.mt * F::kRows + row;
     const bool there = of < n_rows;
     const int t = a.by_group(of), hd = of - t * a.group;
-    const float unit = F::F8 ? v_ref * (1.f / kPScale) : 1.f, by = !complete ? unit : l == 0.f ? 0.f : unit / l;
+    const float unit = F::F8 ? 1.f / f : 1.f, by = !complete ? unit : l == 0.f ? 0.f : unit / l;
     bf16* out = a.out + (size_t)(done.s.row + t) * a.ld_out + (size_t)(done.head * a.group + hd) * HD;
     if (!complete && there) a.stats[(size_t)slot * F::kRows + row] = make_float2(limit == -INFINITY ? -INFINITY : base, l);
 #pragma unroll 1
@@ -511,7 +512,7 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
       tmem_ld_32x16(tmem_o + x, o);
       tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] *= by;
+      for (int e = 0; e < 16; ++e) o[e] *= by, o[e] *= unit;
       if (!there) {
       } else if (complete) {
 #pragma unroll

@@ -1,0 +1,56 @@
+"""Serving operators where their inputs are legal but far from ordinary: scales that differ by powers of two without end, hidden pages, draws
+at the ends of their range, places that nothing fits."""
+import pytest
+import torch
+from serving_utils import Cache, attention, attention_exact, attention_tolerance, i32, status
+from test_serving_gpu import check_attention
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- scales of values -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new", [1, 4, 40, 100])
+@pytest.mark.parametrize("window", [0, 70])
+def test_attention_scales_of_pages_that_a_row_does_not_see(page, new, window):
+    """Values 2^30 times the others', ahead of all rows but the last ones and, with a window, behind all but the first ones."""
+    pos = 200
+    cache = Cache([pos + new], 2, 64, page, "e4m3", seed=4)
+    loud = {(pos + new - 1) // page} if new > 1 else set()
+    if window:
+        loud.add((pos + 1 - window) // page)
+    for slot in loud:
+        cache.vs[cache.table_host[0][slot]] *= 2.0 ** 30
+    check_attention("e4m3", 4, 2, 64, page, [new], [pos], window=window, cache=cache)
+
+
+@pytest.mark.parametrize("new", [1, 8, 100])
+@pytest.mark.parametrize("ratio", [26, 30, 36, 100])
+@pytest.mark.parametrize("first", [True, False])
+def test_attention_concentrated_on_pages_of_small_scales(new, ratio, first):
+    """A row whose probabilities lie on pages with values far smaller than those of others that it sees: 48 in the exponent less there, or 96 where
+    the values differ by more than that outweighs."""
+    heads, kv, hd, page, pos = 2, 1, 64, 16, 300
+    n = pos + new
+    cache = Cache([n], kv, hd, page, "e4m3", seed=6)
+    sign = torch.where(torch.rand(hd, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0)
+    # scores are 64 * 0.25 * 8^-1 = 2 times a key's size: 0 and 0.875 on ordinary pages
+    size = torch.where(torch.rand(n, generator=torch.Generator().manual_seed(2)) < 0.5, 0.0, 0.4375)
+    large = range(0, 6) if first else range(10, 16)
+    for slot in large:
+        size[slot * page:(slot + 1) * page] = -24.0 if ratio < 60 else -48.0
+        cache.vs[cache.table_host[0][slot]] *= 2.0 ** ratio
+    cache.ks.fill_(1.0)
+    rows = (size[:, None] * sign).to(torch.float8_e4m3fn)
+    for p in range(n):
+        cache.k[cache.table_host[0][p // page], (p % page) * hd:(p % page + 1) * hd] = rows[p].cuda()
+    q = (0.25 * sign).repeat(new, heads).to(torch.bfloat16).cuda()
+    out = torch.full_like(q, 7.0)
+    attention(cache, heads, q, out, i32([0, new]), i32([pos]), new)
+    assert status() == 0
+    k, v = cache.rows("k", 0, n), cache.rows("v", 0, n)
+    mq = q.double().cpu().view(new, heads, hd)
+    ref, mass, big = attention_exact(mq, k, v, pos, hd ** -0.5, 0)
+    tol = attention_tolerance(ref, mass, big, "e4m3", hd, n, mq, hd ** -0.5, float(k.abs().max()))
+    got = out.double().cpu().view(new, heads, hd)
+    assert ((got - ref).abs() <= tol).all(), float((got - ref).norm() / ref.norm())
