@@ -618,8 +618,8 @@ __device__ __forceinline__ void take_keys(const char* ring, const float4* scales
       }
       r.l[n][h] += sum;  // the thread's own keys; joined at the end
     }
-    // Probabilities in 16 bits.  f16 is finer than the output's type.  bf16 is as coarse, and errors of both add up to 1.4 times the output's own;
-    // where products cost nothing, for few rows, what rounding has left of it is added.
+    // Probabilities in 16 bits.  f16 is finer than the output's type.  bf16 is as coarse, and errors of both add up to 1.4 times the output's own:
+    // what rounding has left of it is added.
 #pragma unroll
     for (int k = 0; k < KG; ++k) {
       if (F8) {

@@ -7,11 +7,12 @@
 //   last         one thread issues the products: the next tile's scores before it waits for this tile's probabilities
 //
 // Probabilities take the place of their scores in tensor memory, in the operands' 16 bits: f16, which is finer than the output's type, for 8-bit
-// pages, bf16 otherwise.  Outputs are renewed only with a row's maximum, which follows its scores with some slack.
+// pages; bf16 otherwise, and behind it what that leaves of them, a second product, without which the error is 1.4 times that of rounding
+// the result.  Outputs are renewed only with a row's maximum, which follows its scores with some slack.
 //
 // The 8192 exponentials of a tile take 512 cycles of an SM at 16 a cycle; the products 256 with heads of 64.  Heads of up to 64 have two CTAs an
 // SM, so that one's waits and copies run under the other's softmax: 850 to 1000 cycles a tile and SM.  Eight sequences of 400 tokens over 1500,
-// 12 heads of 64 with 4 for keys: 49 us from 8-bit pages and 41 from bf16 (8.2 GFLOP; by mma.sync, every warp converting all keys, 74 and 59),
+// 12 heads of 64 with 4 for keys: 48 us from 8-bit pages and 45 from bf16, 41 without the second product (8.2 GFLOP; by mma.sync, every warp converting all keys, 74 and 59),
 // of which 4 go into cutting the work and 8 into joining shared items; two of 100 over 60000, 16 heads of 128 with 2, 161 and 127 (334 by
 // mma.sync).  Two threads a row, with half of the keys each, took 60 and 49 in place of 52 and 45: registers for 22 warps are too few; half of the
 // scores loaded under the maximum of the others 50.4 and 42.6 in place of 49.2 and 41.6.
@@ -24,7 +25,7 @@ namespace {
 template <int HD_, bool F8_>
 struct Prompt {
   static constexpr int HD = HD_;
-  static constexpr bool F8 = F8_, kSplit = false;
+  static constexpr bool F8 = F8_, kSplit = false, kRest = !F8_;  // probabilities have one
   // copying warps: two are all that the registers of two CTAs allow; 60000 tokens of heads of 128 took 213 us with two, 184 with four
   static constexpr int kLoaders = HD <= 64 ? 2 : 4, kEach = 4 / kLoaders, kWarps = 5 + kLoaders, kThreads = 32 * kWarps;
   static constexpr int kRows = 128, kTile = 64, kCtas = HD <= 64 ? 2 : 1;
@@ -313,9 +314,12 @@ __device__ __forceinline__ void prompt_issue(const Attn& a, const Plan& plan, It
       if (*reinterpret_cast<const volatile uint32_t*>(m.odd[n % F::kInfo]) == 0) {
         const uint32_t v = tiles + n % F::kStages * F::kStage + F::kX;
 #pragma unroll
-        for (int x = 0; x < F::kTile / 16; ++x)
-          tc_mma_from_tmem(tmem + 2 * F::kTile, tmem + (n & 1) * F::kTile + x * 8, make_smem_desc(v + x * 2048, F::kAtomX, 1024), for_outputs,
-                           i > 0 || x > 0 ? 1u : 0u);
+        for (int x = 0; x < F::kTile / 16; ++x) {
+          const uint64_t values = make_smem_desc(v + x * 2048, F::kAtomX, 1024);
+          const uint32_t p = tmem + (n & 1) * F::kTile + x * 8;
+          tc_mma_from_tmem(tmem + 2 * F::kTile, p, values, for_outputs, i > 0 || x > 0 ? 1u : 0u);
+          if (F::kRest) tc_mma_from_tmem(tmem + 2 * F::kTile, p + F::kTile / 2, values, for_outputs, 1u);
+        }
       }
       tc_commit(smem_u32(&m.outputs[n & 1]));
       tc_commit(smem_u32(&m.empty[n % F::kStages]));
@@ -429,8 +433,8 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
         }
       }
       uint64_t sums[2] = {0, 0};
-      uint32_t p[kTile / 2];
-      const uint64_t less = both(-base, -base);
+      uint32_t p[kTile / 2], rest[F::kRest ? kTile / 2 : 1];
+      const uint64_t less = both(-base, -base), minus = both(-1.f, -1.f);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const uint64_t by = both(mults[g], mults[g]);
@@ -444,6 +448,11 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
           if (F::F8) two = mul_both(two, both(into[g], into[g]));
           each(two, lo, hi);
           p[e] = pack<F::F8>(lo, hi);
+          if constexpr (F::kRest) {
+            float lo_left, hi_left;
+            each(fma_both(both(__uint_as_float(p[e] << 16), __uint_as_float(p[e] & 0xffff0000u)), minus, two), lo_left, hi_left);
+            rest[e] = pack<false>(lo_left, hi_left);
+          }
         }
       }
       {
@@ -453,6 +462,7 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
       }
       // The place is free: the products with the tile before last were complete before this one's scores.
       tmem_st_32x32(tmem + (n & 1) * kTile, p);
+      if constexpr (F::kRest) tmem_st_32x32(tmem + (n & 1) * kTile + kTile / 2, rest);
       tmem_st_wait();
       if (odd) {
         // A value that is infinite or NaN must not reach rows that do not see its key, and 0 * NaN is NaN: one product after the other, unseen
@@ -475,8 +485,10 @@ __device__ __forceinline__ void prompt_rows(const Attn& a, const Plan& plan, Ite
 #pragma unroll 1
           for (int key = 0; key < kTile; ++key) {
             const uint32_t two = tmem_ld_32x1(tmem + (n & 1) * kTile + key / 2);
+            const uint32_t left = F::kRest ? tmem_ld_32x1(tmem + (n & 1) * kTile + kTile / 2 + key / 2) : 0u;
             tmem_ld_wait();
-            const float w = from_16<F::F8>((uint16_t)(key & 1 ? two >> 16 : two));
+            float w = from_16<F::F8>((uint16_t)(key & 1 ? two >> 16 : two));
+            if (F::kRest) w += from_16<false>((uint16_t)(key & 1 ? left >> 16 : left));
             const bool seen = key0 + key <= pos && !(a.window && key0 + key <= pos - a.window);
 #pragma unroll
             for (int e = 0; e < 16; ++e)

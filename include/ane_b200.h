@@ -182,9 +182,9 @@ int32_t ane_op_kv_append(const ane_kv_append_args* args);
 
 /* Attention of new tokens over their sequences' caches, the new tokens' own keys included (append first): the token at
  * position p sees positions 0 .. p, with a window only the last `window` of them.  One token a sequence or many.  Softmax statistics
- * and sums in fp32, probabilities enter their product in 16 bits (over bf16 pages, where max_new * n_heads / n_kv_heads is at most 32,
- * with what that leaves of them; over 8-bit pages a probability times its page's scale of values counts as nothing where that is below
- * about 2^-31 of the largest such product that the row sees).  Results are the same from call to call. */
+ * and sums in fp32, probabilities enter their product in 16 bits: over bf16 pages with what that leaves of them, over 8-bit pages times
+ * their page's scale of values, where a product below about 2^-31 of the largest that the row sees counts as nothing.  Results are the same
+ * from call to call. */
 typedef struct ane_kv_attention_args {
   uint32_t struct_size;
   int32_t n_heads;

@@ -54,3 +54,19 @@ def test_attention_concentrated_on_pages_of_small_scales(new, ratio, first):
     tol = attention_tolerance(ref, mass, big, "e4m3", hd, n, mq, hd ** -0.5, float(k.abs().max()))
     got = out.double().cpu().view(new, heads, hd)
     assert ((got - ref).abs() <= tol).all(), float((got - ref).norm() / ref.norm())
+
+
+# ---- probabilities --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hd", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("new", [1, 12, 90])
+def test_attention_is_as_exact_with_many_rows_as_with_few(kind, hd, new):
+    """What is left of the error is the result's rounding: probabilities enter with errors of 2^-16 (bf16 with a rest) or 2^-12 (f16), against 2^-8 at
+    most, so that the error's norm exceeds the rounding's by less than one in a hundred; a twentieth is granted."""
+    heads, kv, pos = 4, 2, 300
+    cache, q, out = check_attention(kind, heads, kv, hd, 64, [new], [pos], loud=2.0)
+    k, v = cache.rows("k", 0, pos + new), cache.rows("v", 0, pos + new)
+    ref, _, _ = attention_exact(q.double().cpu().view(new, heads, hd), k, v, pos, hd ** -0.5, 0)
+    off = (out.double().cpu().view(new, heads, hd) - ref).norm()
+    rounding = (ref.to(torch.bfloat16).double() - ref).norm()
+    assert off <= 1.05 * rounding, float(off / rounding)
