@@ -977,7 +977,8 @@ void argmax_rows(const float* logits, int32_t* out, int rows, int V, cudaStream_
 // result = first i whose running sum reaches target.  One block per row: every thread owns a contiguous chunk and
 // sums it in index order, thread 0 scans the 256 chunk sums in order, and the thread whose chunk straddles the
 // target walks it again.  The running sum therefore groups the additions by chunk; the index can differ from the
-// reference's single serial sum only when target lies within double rounding of a prefix boundary.
+// reference's single serial sum only when target lies within double rounding of a prefix boundary.  A token without weight (a logit of
+// -infinity, as masks leave it) is not drawn while another has some: neither for target == 0, nor where sums round below the target.
 __global__ void __launch_bounds__(256)
 sample_rows_kernel(const float* __restrict__ logits, const double* __restrict__ u, float temperature,
                    int32_t* __restrict__ out, int rows, int V) {
@@ -987,10 +988,11 @@ sample_rows_kernel(const float* __restrict__ logits, const double* __restrict__ 
   __shared__ float s_max[256];
   __shared__ double s_sum[256];
   __shared__ double s_target;
-  __shared__ int s_pick;
+  __shared__ int s_pick, s_last;
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < V; i += blockDim.x) mx = fmaxf(mx, p[i]);
   s_max[threadIdx.x] = mx;
+  if (threadIdx.x == 0) s_last = -1;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
     if ((int)threadIdx.x < o) s_max[threadIdx.x] = fmaxf(s_max[threadIdx.x], s_max[threadIdx.x + o]);
@@ -1001,8 +1003,14 @@ sample_rows_kernel(const float* __restrict__ logits, const double* __restrict__ 
   const int per = (V + 255) / 256;
   const int i0 = min((int)threadIdx.x * per, V), i1 = min(i0 + per, V);
   double part = 0.0;
-  for (int i = i0; i < i1; ++i) part += exp(((double)p[i] - maxv) * inv_temp);
+  int last = -1;  // of the chunk's tokens with weight
+  for (int i = i0; i < i1; ++i) {
+    const double e = exp(((double)p[i] - maxv) * inv_temp);
+    part += e;
+    if (e > 0.0) last = i;
+  }
   s_sum[threadIdx.x] = part;
+  if (last >= 0) atomicMax(&s_last, last);
   __syncthreads();
   if (threadIdx.x == 0) {
     double acc = 0.0;
@@ -1012,19 +1020,21 @@ sample_rows_kernel(const float* __restrict__ logits, const double* __restrict__ 
       acc += v;
     }
     s_target = u[row] * acc;
-    s_pick = V - 1;  // the reference's answer when the running sum never reaches target
+    // the reference's answer when the running sum never reaches target, which a sum that is NaN does not
+    s_pick = acc == acc && s_last >= 0 ? s_last : V - 1;
   }
   __syncthreads();
   const double target = s_target;
   const double before = s_sum[threadIdx.x];
   const double through = before + part;
-  // exactly one chunk has before < target <= through, except at target == 0 (the first element wins)
-  if (i1 > i0 && through >= target && (before < target || threadIdx.x == 0)) {
+  // exactly one chunk has before < target <= through, except at target == 0 (the first element with weight wins)
+  if (last >= 0 && through >= target && (before < target || before == 0.0)) {
     double acc = before;
-    int pick = i1 - 1;
+    int pick = last;
     for (int i = i0; i < i1; ++i) {
-      acc += exp(((double)p[i] - maxv) * inv_temp);
-      if (acc >= target) {
+      const double e = exp(((double)p[i] - maxv) * inv_temp);
+      acc += e;
+      if (e > 0.0 && acc >= target) {
         pick = i;
         break;
       }

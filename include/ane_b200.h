@@ -60,6 +60,7 @@ int32_t ane_op_cast_f32_to_bf16(const float* d_src, void* d_dst, uint64_t n);
 int32_t ane_op_cast_bf16_to_f32(const void* d_src, float* d_dst, uint64_t n);
 /* sampleFromLogits (ane/train_full.go:318-342) for `rows` rows of `vocab` fp32 logits: d_out[r] = sampled
  * index of row r for the uniform draw d_u[r]; temperature <= 1e-6 gives argmax (ane/train_full.go:344-354).
+ * A token without weight, as one whose logit is -infinity, is not drawn while another has some.
  * All three pointers are device pointers. */
 int32_t ane_op_sample_rows(const float* d_logits, const double* d_u, float temperature, int32_t* d_out, int32_t rows,
                            int32_t vocab);

@@ -1,8 +1,13 @@
 """Serving operators where their inputs are legal but far from ordinary: scales that differ by powers of two without end, hidden pages, draws
 at the ends of their range, places that nothing fits."""
+import math
+
+import numpy as np
 import pytest
 import torch
-from serving_utils import Cache, attention, attention_exact, attention_tolerance, i32, status
+from oracle import oracle as O
+from serving_utils import Cache, attention, attention_exact, attention_tolerance, i32, lib, ptr, rules, status
+from test_generate_gpu import pair
 from test_serving_gpu import check_attention
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +75,53 @@ def test_attention_is_as_exact_with_many_rows_as_with_few(kind, hd, new):
     off = (out.double().cpu().view(new, heads, hd) - ref).norm()
     rounding = (ref.to(torch.bfloat16).double() - ref).norm()
     assert off <= 1.05 * rounding, float(off / rounding)
+
+
+# ---- draws among masked logits --------------------------------------------------------------------------------------------------
+ENDS = [0.0, 5e-324, 2.0 ** -60, 1.0 - 2.0 ** -53]
+
+
+def sample(logits, u, temperature):
+    out = torch.full((logits.shape[0],), -7, dtype=torch.int32, device="cuda")
+    assert lib.ane_op_sample_rows(ptr(logits), ptr(u), temperature, ptr(out), *logits.shape) == 0, lib.ane_ops_last_error()
+    return out.cpu().numpy()
+
+
+@pytest.mark.parametrize("temperature", [0.3, 1.0, 7.0])
+@pytest.mark.parametrize("vocab,away", [(2, [0]), (2, [1]), (7, [0, 6]), (600, [0, 1, 2, 3, 597, 598, 599]), (32000, [*range(300), 5000, *range(31500, 32000)])])
+def test_sampler_does_not_draw_what_a_mask_forbids(vocab, away, temperature):
+    """Rules and then the sampler, with draws at both ends: the first and the last token with weight, and no token without."""
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy((3 * rng.standard_normal((len(ENDS) + 20, vocab))).astype(np.float32)).cuda()
+    u = np.concatenate([ENDS, rng.random(20)])
+    words = np.full((vocab + 31) // 32, 0xffffffff, dtype=np.uint32)
+    for v in away:
+        words[v // 32] &= ~np.uint32(1 << v % 32)
+    rules(x, x, d_mask=torch.from_numpy(words.view(np.int32)).cuda(), ld_mask=len(words), n_masks=1, d_mask_row=i32([0] * len(u)))
+    got = sample(x, torch.from_numpy(u).cuda(), temperature)
+    may = np.setdiff1d(np.arange(vocab), away)
+    assert np.isin(got, may).all(), got
+    assert got[0] == may[0] and got[1] == may[0]
+    assert got[3] == may[-1] or vocab > 7  # the last token's weight may be below the draw's distance from 1
+
+
+def test_sampler_without_masks_draws_what_it_drew():
+    x = torch.full((5, 1000), 0.5, device="cuda")
+    x[4] = math.nan
+    got = sample(x, torch.tensor([0.0, 1e-300, 0.5, 1.0 - 2.0 ** -53, 0.5], dtype=torch.float64, device="cuda"), 1.0)
+    assert got.tolist() == [0, 0, 499, 999, 999]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_generate_draws_allowed_tokens_only(kv):
+    cfg, e = pair(vocab=512)
+    allowed = np.random.default_rng(4).random(cfg["vocab"]) < 0.4
+    allowed[[0, 1, cfg["vocab"] - 1]] = False
+    prompts = [O.zipf_tokens(n, cfg["vocab"], n) for n in (40, 3, 17)]
+    for end in ENDS:
+        got = e.generate(prompts, 12, kv=kv, temperature=1.0, uniforms=np.full((12, 3), end), allowed=allowed)
+        assert allowed[got].all(), (end, got)
+    # without a mask, a draw of 0 is the first token
+    got = e.generate(prompts, 6, kv=kv, temperature=1.0, uniforms=np.zeros((6, 3)), bias={7: 5.0})
+    assert (got == 0).all()
+    e.close()
