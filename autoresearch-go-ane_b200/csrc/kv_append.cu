@@ -29,7 +29,8 @@ struct Append {
   const bf16* qkv;  // may be q: every element is read by the thread that writes it
   bf16* q;
   const float *cosb, *sinb;
-  int ld_qkv, ld_q, heads, n_positions;
+  int ld_qkv, ld_q, heads;
+  int n_positions;  // that may be written: those of the tables, or any
   int rows_blocks;  // blocks that rotate rows; the others are 8-bit pages
   int units;        // bound of the pages that are touched
   int capacity;     // tokens of a sequence
@@ -136,7 +137,7 @@ __device__ __forceinline__ void append_rows(const Append& a, int block) {
       }
     if (b == a.batch.n_seq || s.n == 0 || row < s.row) continue;
     const int pos = s.pos + row - s.row;
-    if (turn && pos >= a.n_positions) {
+    if (pos >= a.n_positions) {
       atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
       continue;
     }
@@ -201,12 +202,10 @@ __device__ __forceinline__ void append_page(const Append& a, int unit, int head,
   if (ahead < 0 || slot > a.by_page(s.pos + s.n - 1)) return;
   const int p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];
   const bool turn = !values && a.cosb;
-  if (turn && s.pos + s.n > a.n_positions) {
-    if (lane == 0) atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
-    return;
-  }
+  if (s.pos + s.n > a.n_positions && lane == 0) atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
   const int page0 = slot * page;
-  const int lo = max(s.pos, page0) - page0, hi = min(s.pos + s.n, page0 + page) - page0;  // new rows of the page
+  const int lo = max(s.pos, page0) - page0, hi = min(min(s.pos + s.n, a.n_positions), page0 + page) - page0;  // new rows of the page
+  if (hi <= lo) return;
   const bf16* in = a.qkv + (size_t)(s.row + page0 + lo - s.pos) * a.ld_qkv + (a.heads + (values ? a.kv.kv_heads : 0) + head) * hd;
   const float* c = turn ? a.cosb + (size_t)(page0 + lo) * half : nullptr;
   const float* n = turn ? a.sinb + (size_t)(page0 + lo) * half : nullptr;
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const Append a) {
 cudaError_t kv_append(const PagedKv& kv, const Batch& batch, int heads, const bf16* qkv, int ld_qkv, bf16* q, int ld_q,
                       const float* cosb, const float* sinb, int n_positions, int* status, cudaStream_t s) {
   if (batch.n_seq == 0 || batch.n_tokens == 0) return cudaSuccess;
-  Append a = {kv, batch, qkv, q, cosb, sinb, ld_qkv, ld_q, heads, n_positions};
+  Append a = {kv, batch, qkv, q, cosb, sinb, ld_qkv, ld_q, heads, cosb ? n_positions : INT32_MAX};
   a.status = status;
   a.capacity = (int)min((long long)kv.table_pitch * kv.page_size, (long long)INT32_MAX);
   a.q_vec = q ? heads * kv.head_dim / 8 : 0;

@@ -171,7 +171,7 @@ typedef struct ane_kv_append_args {
   int32_t ld_qkv, ld_q;      /* multiples of 8 */
   const float* d_cos;        /* [n_positions][head_dim / 2]; both NULL: no rotation */
   const float* d_sin;
-  int32_t n_positions;
+  int32_t n_positions;       /* of the tables: a token behind them is out of range, its query and value too */
   int32_t n_seq;
   const int32_t* d_seq_start;
   const int32_t* d_pos;

@@ -6,9 +6,10 @@ import numpy as np
 import pytest
 import torch
 from oracle import oracle as O
-from serving_utils import Cache, attention, attention_exact, attention_tolerance, i32, lib, ptr, rules, status
+from serving_utils import (BAD_INDEX, Cache, append, attention, attention_exact, attention_tolerance, i32, lib, ptr, rope_tables, rules, starts,
+                           status)
 from test_generate_gpu import pair
-from test_serving_gpu import check_attention
+from test_serving_gpu import KINDS, check_attention, qkv_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -62,7 +63,7 @@ def test_attention_concentrated_on_pages_of_small_scales(new, ratio, first):
 
 
 # ---- probabilities --------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [32, 48, 64, 96, 128])
 @pytest.mark.parametrize("new", [1, 12, 90])
 def test_attention_is_as_exact_with_many_rows_as_with_few(kind, hd, new):
@@ -112,7 +113,7 @@ def test_sampler_without_masks_draws_what_it_drew():
     assert got.tolist() == [0, 0, 499, 999, 999]
 
 
-@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("kv", KINDS)
 def test_generate_draws_allowed_tokens_only(kv):
     cfg, e = pair(vocab=512)
     allowed = np.random.default_rng(4).random(cfg["vocab"]) < 0.4
@@ -125,3 +126,33 @@ def test_generate_draws_allowed_tokens_only(kv):
     got = e.generate(prompts, 6, kv=kv, temperature=1.0, uniforms=np.zeros((6, 3)), bias={7: 5.0})
     assert (got == 0).all()
     e.close()
+
+
+# ---- places that nothing fits ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,pos", [([1, 1, 1], [18, 19, 20]), ([15], [10]), ([3], [16]), ([30, 2], [0, 25]), ([40, 1], [15, 19])])
+def test_append_behind_the_rotation_tables_is_not_written(kind, new, pos):
+    """Tables of 20 positions, a cache of more: what lies within them is appended as if the other tokens were not there, which leave queries, keys,
+    values and scales as they are."""
+    heads, kv, hd, page, n_positions = 4, 2, 64, 16, 20
+    cos, sin = rope_tables(n_positions, hd)
+    start = starts(new)
+    qkv = qkv_rows(start[-1], heads, kv, hd, 3)
+    fits = [max(0, min(n, n_positions - p)) for n, p in zip(new, pos)]
+    results = []
+    for lens in (new, fits):
+        cache = Cache([60, 60, 60][:len(new)], kv, hd, page, kind, seed=2)
+        q = torch.full((start[-1], heads * hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        if lens is new:
+            append(cache, heads, qkv, q, i32(start), i32(pos), cos, sin)
+        else:
+            for b, n in enumerate(fits):  # one sequence after the other: their rows are not next to one another
+                if n == 0:
+                    continue
+                one = Cache([60, 60, 60][:len(new)], kv, hd, page, kind, seed=2)
+                one.k, one.v, one.ks, one.vs, one.table = cache.k, cache.v, cache.ks, cache.vs, cache.table[b:b + 1].contiguous()
+                rows = slice(start[b], start[b] + n)
+                append(one, heads, qkv[rows], q[rows], i32([0, n]), i32([pos[b]]), cos, sin)
+        assert status() == (BAD_INDEX if lens is new and fits != new else 0)  # 16 .. 18 fit
+        results.append([q, cache.k.view(torch.uint8), cache.v.view(torch.uint8)] + ([cache.ks, cache.vs] if kind == "e4m3" else []))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
