@@ -23,6 +23,7 @@ static thread_local std::string g_ops_err;
 // One device status word and one timer event pair per device: a kernel launched on device d must be handed
 // device-d memory, and events belong to the device that was current when they were made.
 static constexpr int kMaxDevices = 64;
+static std::mutex g_status_mutex;
 static int* g_ops_status_dev[kMaxDevices] = {nullptr};
 static cudaEvent_t g_ev0_dev[kMaxDevices] = {nullptr}, g_ev1_dev[kMaxDevices] = {nullptr};
 // Room for the parts of an fp32 product's operands, one block per device, taken with the first such product and kept, so that a call
@@ -54,14 +55,20 @@ static int current_device(int* dev) {
   if (*dev < 0 || *dev >= kMaxDevices) return set_err(ANE_ERR_ARG, "device ordinal out of range");
   return 0;
 }
-// The status word of the current device (allocated on first use there).
+// Clears a status word; when this returns it is clear, for kernels on any stream.
+static cudaError_t clear_status(int* p) {
+  const cudaError_t e = cudaMemset(p, 0, sizeof(int));
+  return e == cudaSuccess ? cudaStreamSynchronize(0) : e;
+}
+// The status word of the current device (allocated on first use there, by one thread).
 static int ensure_status(int** out) {
   int dev = 0;
   if (int rc = current_device(&dev)) return rc;
+  std::lock_guard<std::mutex> lock(g_status_mutex);
   if (!g_ops_status_dev[dev]) {
     int* p = nullptr;
     CK(cudaMalloc(&p, sizeof(int)));
-    cudaError_t e = cudaMemset(p, 0, sizeof(int));
+    const cudaError_t e = clear_status(p);
     if (e != cudaSuccess) {
       cudaFree(p);
       return cuda_fail(e, "cudaMemset");
@@ -151,7 +158,7 @@ int32_t ane_ops_device_status(int32_t* out_status) {
   if (ensure_status(&status)) return ANE_ERR_CUDA;
   int v = 0;
   CK(cudaMemcpy(&v, status, sizeof(int), cudaMemcpyDeviceToHost));
-  CK(cudaMemset(status, 0, sizeof(int)));
+  if (v != 0) CK(clear_status(status));
   if (out_status) *out_status = v;
   return 0;
 }

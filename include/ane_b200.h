@@ -54,6 +54,8 @@ int32_t ane_dev_sync(void);
 int32_t ane_timer_begin(void);
 int32_t ane_timer_end(float* out_ms);
 const char* ane_ops_last_error(void);
+/* What the kernels of the calls so far have reported on the current device, 0: nothing; and clears it.  Waits for the default stream: a stream
+ * that does not wait for that one has to be synchronised first. */
 int32_t ane_ops_device_status(int32_t* out_status);
 
 int32_t ane_op_cast_f32_to_bf16(const float* d_src, void* d_dst, uint64_t n);

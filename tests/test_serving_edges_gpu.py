@@ -1,6 +1,9 @@
 """Serving operators where their inputs are legal but far from ordinary: scales that differ by powers of two without end, hidden pages, draws
 at the ends of their range, places that nothing fits."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -156,3 +159,35 @@ def test_append_behind_the_rotation_tables_is_not_written(kind, new, pos):
         assert status() == (BAD_INDEX if lens is new and fits != new else 0)  # 16 .. 18 fit
         results.append([q, cache.k.view(torch.uint8), cache.v.view(torch.uint8)] + ([cache.ks, cache.vs] if kind == "e4m3" else []))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+FIRST_CALLS = """
+import sys, threading
+sys.path[:0] = sys.argv[1:]
+import conftest, torch
+from serving_utils import Cache, attention_args, i32, lib, status, workspace, BAD_INDEX
+import ctypes
+cache = Cache([32], 1, 64, 16, "bf16")
+q = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+out, work = torch.zeros_like(q), workspace(1, 1, 64)
+start, pos = i32([0, 4]), i32([-3])
+streams = [torch.cuda.Stream() for _ in range(8)]
+args = [attention_args(cache, 1, q, out, start, pos, 4, work=torch.empty_like(work), stream=s.cuda_stream) for s in streams]
+torch.cuda.synchronize()
+torch.cuda._sleep(200_000_000)  # the default stream is busy for a tenth of a second
+threads = [threading.Thread(target=lambda a=a: lib.ane_op_kv_attention(ctypes.byref(a))) for a in args]
+for t in threads: t.start()
+for t in threads: t.join()
+for s in streams: s.synchronize()
+assert status() == BAD_INDEX
+assert status() == 0
+"""
+
+
+def test_first_calls_on_busy_devices_and_several_threads_keep_their_reports():
+    """The status word is taken by the first call of a process: on streams that do not wait for the default one, while that one is busy."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    root = os.path.dirname(here)
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS, here, root, os.path.join(root, "autoresearch-go-ane_b200")], capture_output=True, text=True,
+                         timeout=300, env=dict(os.environ, CUDA_MODULE_LOADING="EAGER"))  # else the first launch waits for the device
+    assert run.returncode == 0, run.stderr[-2000:]
