@@ -11,7 +11,7 @@ import torch
 from oracle import oracle as O
 from serving_utils import (BAD_INDEX, Cache, append, attention, attention_exact, attention_tolerance, i32, lib, ptr, rope_tables, rules, starts,
                            status)
-from test_generate_gpu import pair
+from test_generate_gpu import CLEAR, forward, pair
 from test_serving_gpu import KINDS, check_attention, qkv_rows
 
 pytestmark = pytest.mark.gpu
@@ -191,3 +191,29 @@ def test_first_calls_on_busy_devices_and_several_threads_keep_their_reports():
     run = subprocess.run([sys.executable, "-c", FIRST_CALLS, here, root, os.path.join(root, "autoresearch-go-ane_b200")], capture_output=True, text=True,
                          timeout=300, env=dict(os.environ, CUDA_MODULE_LOADING="EAGER"))  # else the first launch waits for the device
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+# ---- generation of many prompts at once -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kv", KINDS)
+def test_generate_of_forty_ragged_prompts_gives_what_each_gives_alone(kv):
+    """More sequences than the dense kernels take.  Each row follows from its own prompt: a token is the best one of a full forward pass but for what
+    bf16 (the margin of the other tests) or 8-bit caches can turn round, and what its prompt gives alone up to the first place where two tokens are
+    as near as that."""
+    cfg, e = pair(batch=40, seq=100, layers=2)
+    prompts = [O.zipf_tokens(1 + 2 * b, cfg["vocab"], b) for b in range(40)]
+    got = e.generate(prompts, 21, kv=kv)
+    same = 0
+    for b, p in enumerate(prompts):
+        alone = e.generate([p], 21, kv=kv)[0]
+        apart = False
+        for i, col in enumerate(forward(e, cfg, p, got[b])):
+            near = CLEAR if kv == "bf16" else 0.5 * float(col.std())
+            assert col.max() - col[got[b, i]] <= near, (b, i)
+            apart = apart or got[b, i] != alone[i]
+            if apart:
+                assert abs(col[got[b, i]] - col[alone[i]]) <= near, (b, i)
+                break
+            same += 1
+    assert same > 40 * 21 // 2, same
+    assert len({tuple(r) for r in got.tolist()}) > 20  # prompts lead to different texts
+    e.close()
