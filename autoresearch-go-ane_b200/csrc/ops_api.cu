@@ -405,7 +405,8 @@ int32_t ane_op_logit_rules(const ane_logit_rules_args* a) {
     if (!a || a->struct_size != sizeof(ane_logit_rules_args)) return *fault = "bad struct_size", ANE_ERR_ARG;
     if (a->dtype != ANE_DTYPE_F32 && a->dtype != ANE_DTYPE_BF16) return *fault = "logits must be fp32 or bf16", ANE_ERR_ARG;
     if (!a->d_logits || !a->d_out) return *fault = "null pointer", ANE_ERR_ARG;
-    if (a->rows < 0 || a->vocab <= 0 || a->ld_logits < a->vocab || a->ld_out < a->vocab) return *fault = "bad dimensions", ANE_ERR_ARG;
+    // kernels step over the vocabulary in 32 bits, some thousand tokens at a time
+    if (a->rows < 0 || a->vocab <= 0 || a->vocab > (1 << 30) || a->ld_logits < a->vocab || a->ld_out < a->vocab) return *fault = "bad dimensions", ANE_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(a->d_logits) % (a->dtype == ANE_DTYPE_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(a->d_out) % 4)
       return *fault = "misaligned logits", ANE_ERR_ARG;
     if (a->d_logits == a->d_out && (a->dtype != ANE_DTYPE_F32 || a->ld_logits != a->ld_out))

@@ -220,7 +220,7 @@ typedef struct ane_logit_rules_args {
   const void* d_logits;      /* [rows][ld_logits] */
   float* d_out;              /* [rows][ld_out]; may be d_logits (fp32, ld_out = ld_logits) */
   int64_t ld_logits, ld_out;
-  int32_t rows, vocab;
+  int32_t rows, vocab;       /* vocab up to 2^30 */
   const int32_t* d_tokens;   /* [rows][ld_tokens]; ids outside the vocabulary are passed over; NULL: no penalties */
   const int32_t* d_n_tokens; /* [rows]: tokens of a row that count, its prompt's and its output's */
   const int32_t* d_n_prompt; /* [rows]: how many of them, from the first, are the prompt's; NULL: none */
