@@ -385,7 +385,8 @@ int32_t ane_op_kv_attention(const ane_kv_attention_args* a) {
     if (a->ld_out < a->n_heads * c.head_dim || a->ld_out % 8) return *fault = "bad ld_out", ANE_ERR_ARG;
     if (a->max_new < 1 || (int64_t)a->max_new * a->n_heads > INT32_MAX) return *fault = "bad max_new", ANE_ERR_ARG;
     if (a->window < 0) return *fault = "bad window", ANE_ERR_ARG;
-    if (!(a->scale >= 0.f && a->scale <= 3.4e38f)) return *fault = "bad scale", ANE_ERR_ARG;
+    if (!(a->scale >= 0.f && a->scale <= 2.3e38f)) return *fault = "bad scale", ANE_ERR_ARG;  // finite in units of log2, too
+    if (a->d_out == a->d_q) return *fault = "the output may not be the queries", ANE_ERR_ARG;
     int* status = nullptr;
     if (ensure_status(&status)) return ANE_ERR_CUDA;
     const uint64_t need = ane_op_kv_attention_workspace(a->n_heads, c.n_kv_heads, c.head_dim);

@@ -201,7 +201,7 @@ typedef struct ane_kv_attention_args {
   int32_t n_tokens;
   int32_t max_new;           /* no sequence has more new tokens than this */
   int32_t window;            /* 0: all positions */
-  float scale;               /* of the scores; 0: head_dim^-1/2 */
+  float scale;               /* of the scores, up to 2.3e38; 0: head_dim^-1/2 */
   int32_t pad_;
   void* d_workspace;         /* 16-byte aligned; for one call at a time, its content does not matter */
   uint64_t workspace_bytes;  /* at least ane_op_kv_attention_workspace() */
