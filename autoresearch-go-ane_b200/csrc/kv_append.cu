@@ -135,7 +135,7 @@ __device__ __forceinline__ void append_rows(const Append& a, int block) {
         end = a.batch.start[b + 1];
         s = span_of(a.batch, b, a.capacity, INT32_MAX, a.status);
       }
-    if (b == a.batch.n_seq || s.n == 0 || row < s.row) continue;
+    if (b == a.batch.n_seq || s.n <= 0 || row < s.row) continue;
     const int pos = s.pos + row - s.row;
     if (pos >= a.n_positions) {
       atomicCAS(a.status, DEV_OK, DEV_BAD_INDEX);
@@ -197,7 +197,7 @@ __device__ __forceinline__ void append_page(const Append& a, int unit, int head,
   const int b = f.b;
   if (b >= a.batch.n_seq) return;
   const Span s = span_of(f.row, f.end, f.pos, a.batch, a.capacity, INT32_MAX, a.status);
-  if (s.n == 0) return;
+  if (s.n <= 0) return;
   const int ahead = unit - (a.by_page(s.row) + 2 * b), slot = a.by_page(s.pos) + ahead;
   if (ahead < 0 || slot > a.by_page(s.pos + s.n - 1)) return;
   const int p = a.kv.table[(size_t)b * a.kv.table_pitch + slot];

@@ -208,7 +208,7 @@ struct Item {
 // How the line of all tiles is cut.  Whole items to a CTA where all are short; one piece of at most `share` tiles of one item to each CTA where
 // that makes the largest share little larger than an even one, since another item costs a CTA a new start; else even shares.
 enum Cut { kWhole, kPieces, kEven };
-// The host has made sure that there are less than 2^31 units.
+// The host has made sure that there are less than 2^31 units where no row belongs to two sequences.
 struct Plan {
   int first, last;  // this CTA's units of the line: items, pieces or tiles
   int share;        // tiles (kWhole: items) of a CTA
@@ -261,11 +261,16 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
   const int split = per > 1 || (F::kSplit && a.one_tile) ? 0 : 31 - __clz(kThreads / a.batch.n_seq), part = tid & ((1 << split) - 1);
   const int b0 = min((tid >> split) * per, a.batch.n_seq), b1 = min(b0 + per, a.batch.n_seq);
   Span s = {0, 0, 0};  // of the thread's only sequence, mostly
+  int longest = 0;     // INT_MIN: starts fall
   // what(tiles of an item) of all items of a KV head of the thread's sequences, until it says stop
   auto each = [&](auto what) {
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       if (per > 1) s = span_of(a.batch, b, a.capacity, a.max_new, a.status);
+      if (s.n < 0) {
+        longest = INT_MIN;
+        return;
+      }
       const int mts = row_tiles<F>(a, s), each_mts = (mts + (1 << split) - 1) >> split, mt1 = min(mts, (part + 1) * each_mts);
 #pragma unroll 1
       for (int mt = part * each_mts; mt < mt1; ++mt)
@@ -273,7 +278,7 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
     }
   };
   if (per == 1 && b0 < b1) s = span_of(a.batch, b0, a.capacity, a.max_new, a.status);
-  int items = 0, tiles = 0, longest = 0;
+  int items = 0, tiles = 0;
   each([&](int, int, int t) {
     ++items;
     tiles += t;
@@ -282,7 +287,7 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
   });
   items = __reduce_add_sync(0xffffffffu, items);
   tiles = __reduce_add_sync(0xffffffffu, tiles);
-  longest = __reduce_max_sync(0xffffffffu, longest);
+  longest = (int)__reduce_max_sync(0xffffffffu, (uint32_t)longest);
   if (lane == 0) all[warp] = make_int3(items, tiles, longest);
   if (tid == 0) at = make_int4(-1, 0, 0, 0);
   __syncthreads();
@@ -291,12 +296,16 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
   for (int w = 0; w < kWarps; ++w) {
     items += all[w].x;
     tiles += all[w].y;
-    longest = max(longest, all[w].z);
+    longest = (int)max((uint32_t)longest, (uint32_t)all[w].z);
+  }
+  Plan p = {};
+  if (longest < 0) {  // reported; rows may belong to several sequences, and nothing bounds the line's length then
+    it.b = -1;
+    return p;
   }
   items *= a.kv.kv_heads;
   tiles *= a.kv.kv_heads;
   const int ctas = gridDim.x;
-  Plan p;
   p.cut = kWhole;
   p.share = quotient_up(items, ctas);
   if (longest > F::kAlone) {

@@ -48,7 +48,7 @@ struct Div {
   }
 };
 
-// New rows and place of sequence b; none (and the status word) where its entries make no sense.
+// New rows and place of sequence b; none (and the status word) where its entries make no sense, n < 0 where its rows would begin behind their end.
 struct Span {
   int row, n, pos;
 };
@@ -56,7 +56,7 @@ __device__ __forceinline__ Span span_of(int row, int end, int pos, const Batch& 
   if (row == end) return {row, 0, pos};
   if (row < 0 || end < row || end > a.n_tokens || end - row > most || pos < 0 || end - row > capacity - pos) {
     atomicCAS(status, DEV_OK, DEV_BAD_INDEX);
-    return {row, 0, pos};
+    return {row, end < row ? -1 : 0, pos};
   }
   return {row, end - row, pos};
 }

@@ -135,7 +135,7 @@ int32_t ane_op_gemm(const ane_gemm_args* args);
  * nor written, and ane_ops_device_status returns 110.  All memory belongs to the current device.
  *
  * A batch: the new tokens of sequence b are the rows d_seq_start[b] .. d_seq_start[b + 1] - 1 (d_seq_start has n_seq + 1
- * entries, no order between sequences' tokens but this one; a sequence may have none), and d_pos[b] tokens are in its cache
+ * entries that never fall; a sequence may have no tokens), and d_pos[b] tokens are in its cache
  * before them, so that row d_seq_start[b] + i has position d_pos[b] + i.  Rows outside all sequences stay as they are. */
 #define ANE_KV_BF16 0
 #define ANE_KV_E4M3 1 /* 8-bit floating point, a scale for each page and head: value = scale * e4m3 */

@@ -161,6 +161,23 @@ def test_append_behind_the_rotation_tables_is_not_written(kind, new, pos):
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_rows_that_many_sequences_claim_is_refused(kind):
+    """Starts that go up and down give every second sequence the same 400 rows: more work than the tokens that the host knows of can be, which is
+    what keeps the line of all tiles within 32 bits."""
+    heads, kv, hd, rows, seqs = 4, 1, 64, 400, 2001
+    cache = Cache([600], kv, hd, 64, kind, seed=5)
+    cache.table = cache.table.expand(seqs, -1).contiguous()
+    q = torch.randn(rows, heads * hd, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    out = torch.full_like(q, 7.0)
+    start = i32([rows * (b % 2) for b in range(seqs + 1)])
+    attention(cache, heads, q, out, start, i32([100] * seqs), rows)
+    assert status() == BAD_INDEX and (out == 7).all()
+    # as many sequences that do not
+    attention(cache, heads, q, out, i32([min(b, rows) for b in range(seqs + 1)]), i32([100] * seqs), rows)
+    assert status() == 0 and not (out == 7).all(1).any()
+
+
 FIRST_CALLS = """
 import sys, threading
 sys.path[:0] = sys.argv[1:]
