@@ -1,8 +1,9 @@
 // Appending keys and values to a paged cache, rotated by their positions on the way (ane_op_kv_append).
 //
 // q|k|v read, rotated q and the cache's rows written, once each: bound by HBM in the limit.  10368 tokens of 32 prompts, 12 + 4 heads of 64 into
-// 8-bit pages take 19.0 us (50 MB, 2.7 TB/s; the floor is 7.7), bound by instructions (40 % of the issue slots) and by the reads that a short
-// block waits for one after the other: sequence, page, rows.  64 single tokens take 3.3 us, one 2.8: launches.
+// 8-bit pages take 18.8 us (50 MB, 2.7 TB/s; the floor is 7.7), into bf16 pages 19.1 (8.5): no pipe is full, 40 % of the issue slots are taken and 33 %
+// of the warps active, so that it is the reads that a short block waits for one after the other: sequence, page, rows.  64 single tokens take
+// 3.3 us, one 2.8: launches.
 #include <cuda_fp8.h>
 
 #include "serving.h"

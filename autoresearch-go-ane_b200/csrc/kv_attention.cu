@@ -16,9 +16,11 @@
 // line, an even share of the line to each CTA of one wave.  What a CTA did of an item that others share goes to the
 // workspace, and a second kernel joins the parts in their order, without atomics: the same sums from call to call.
 //
-// Single tokens, 32 heads of 128 with 8 for keys, 64 sequences of up to 8000 tokens: 208 us from bf16 pages (6.5 TB/s, the memory's rate), 118 to
-// 128 from 8-bit ones (5.3 to 5.7 TB/s; the floor is 103), where instructions that widen, scale and exponentiate bound it.  Small calls are
-// launches and dependent reads: one sequence of 256 tokens 5.7 us, 32 of 768 8.9, two of 60000 with two KV heads 19.8 (the floor is 7.3).
+// Single tokens, 32 heads of 128 with 8 for keys, 64 sequences of up to 8000 tokens: 208 to 213 us from bf16 pages (6.4 TB/s, about the
+// memory's rate), 125 to 132 from 8-bit ones (5.1 to 5.4 TB/s; the floor is 103).  There widening, scaling and exponentials are chains that six
+// warps do not cover: 35 % of the issue slots are taken, 17 % of the warps active, no pipe full.  Small calls are launches and dependent reads: one
+// sequence of 256 tokens 5.8 us, 32 of 768 8.9, two of 60000 with two KV heads 19.7 (the floor is 7.3).  Tables of more than 768 tokens add the
+// launch of the joining kernel, whatever the sequences hold: with 8192, 8.1 and 11.5 us.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -67,13 +69,13 @@ template <int HD, bool F8>
 struct Layout {
   static constexpr int ES = F8 ? 1 : 2;
   static constexpr int RB = HD * ES, GB = kGroup * RB, CPR = RB / 16;  // bytes of a row, of 16 rows; 16-byte pieces of a row
-  static constexpr int VK = RB % 64 == 0 ? 16 : RB % 32 == 0 ? 8 : 4;   // bytes that a thread loads of K rows at a time
-  static constexpr int VV = RB % 128 == 0 ? 16 : RB % 64 == 0 ? 8 : RB % 32 == 0 ? 4 : 2;  // of V rows
+  // 8 bits: bytes that a thread loads of K rows at a time, and of V rows
+  static constexpr int VK = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4, VV = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : HD % 32 == 0 ? 4 : 2;
 };
 
 // A form for few rows: the warps share 8 * NB rows and take a part of the keys each, so that no warp is without rows.
 // Eight warps, but six where 8-bit pages and 128 * 8 outputs a warp do not fit the 128 registers that two CTAs of eight leave: 64 sequences of
-// 8192 tokens with heads of 128 take 118 us (5.7 TB/s) with 168 registers, 126 us with 128 and spills (heads of 64 and 16 rows: 166 and 168).
+// 8000 tokens with heads of 128 take 125 us with 168 registers, 130 us with 128 and spills (heads of 64 and 12 rows, 8192 tokens: 68 and 73).
 // kGroups: times 16 keys that a warp takes at once.  More keys share their softmax's maximum, exchanges and loop, fewer leave the ring room
 // for more stages.
 template <int HD_, bool F8_, int NB_>
@@ -94,9 +96,15 @@ struct Form {
   static constexpr int kMost = 216 * 1024 / kStage, kDeep = kMost > 8 ? 8 : kMost < kStages ? kStages : kMost;  // where a CTA has an SM to itself
   static constexpr int kMostSmem = kDeep * kStage;
   static_assert(kWarps * kRows * HD * 4 <= 3 * kStage, "the warps' outputs are joined in the ring");
-  // Tiles of an item that are not worth sharing (joining parts takes a second kernel), and the least share of one that is shared.
+  // Tiles of an item that are not worth sharing (joining parts takes a second kernel), the least share of one that is shared, and what another
+  // item costs a CTA, as 768, 256 and 768 keys.  us at half and at twice as many beside it, tables as long as the sequences (12 heads of 64 bf16;
+  // A with 4 for keys; B 32 heads of 128 with 8, 8 bits):
+  //   alone    one of 500 9.3 7.7 7.7, of 1500 9.4 9.4 12.0; A 32 of 600 11.4 8.4 8.4, of 1500 14.7 14.7 12.7; B 4 of 700 11.6 12.9 12.9,
+  //            of 1500 13.5 13.5 18.2: few sequences would rather have less, many more
+  //   least    one of 1000 9.6 9.4 10.4, of 1500 10.2 9.4 10.4, of 3000 11.1 11.1 10.6; B 4 of 1000 12.0 12.0 13.4
+  //   restart  (256, 768, 1536) A 32 of 1500 15.5 14.7 14.7; B 16 of 4000 28.6 28.6 34.3, 12 of 8000 36.6 36.6 41.2
   static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile;
-  static constexpr int kRestart = 768 / kTile;  // what another item costs a CTA, in tiles
+  static constexpr int kRestart = 768 / kTile;
 };
 
 // Where 16-byte piece c of a row lies within 16 rows, so that what is read together lies in different banks.  bf16: the same piece of eight
@@ -310,10 +318,16 @@ __device__ __forceinline__ Plan make_plan(const Attn& a, Item& it) {
   p.share = quotient_up(items, ctas);
   if (longest > F::kAlone) {
     const int even = max(quotient_up(tiles, ctas), F::kLeast);
-    // at most tiles / share + items pieces
-    const int pieces = items < ctas ? max(quotient_up(tiles, ctas - items), even) : INT32_MAX;
-    p.cut = F::kSplit && pieces <= even + F::kRestart ? kPieces : kEven;
-    p.share = p.cut == kPieces ? pieces : even;
+    p.cut = kEven;
+    p.share = even;
+    if constexpr (F::kSplit) {
+      // at most tiles / share + items pieces
+      const int pieces = items < ctas ? max(quotient_up(tiles, ctas - items), even) : INT32_MAX;
+      if (pieces <= even + F::kRestart) {
+        p.cut = kPieces;
+        p.share = pieces;
+      }
+    }
   }
   auto weight = [&](int t) { return p.cut == kWhole ? 1 : p.cut == kPieces ? quotient_up(t, p.share) : t; };
   int mine = 0;
@@ -486,7 +500,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 template <int HD, bool F8>
 __device__ __forceinline__ int column(int x, int g) {
   using L = Layout<HD, F8>;
-  constexpr int EV = L::VV / L::ES;
+  constexpr int EV = L::VV;
   return F8 ? x / EV * 8 * EV + g * EV + x % EV : 8 * x + g;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t w) {  // of an 8 x 8 matrix of 16-bit values
@@ -684,7 +698,7 @@ __device__ __forceinline__ void take_keys(const char* ring, const float4* scales
       return;
     }
   }
-  constexpr int EV = L::VV / L::ES, WV = L::VV >= 4 ? L::VV / 4 : 1;
+  constexpr int EV = L::VV, WV = L::VV >= 4 ? L::VV / 4 : 1;
 #pragma unroll
   for (int k = 0; k < KG; ++k) {
     const char* vs = ring + k * 2 * L::GB + L::GB;

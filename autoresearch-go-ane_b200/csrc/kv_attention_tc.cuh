@@ -10,12 +10,13 @@
 // pages; bf16 otherwise, and behind it what that leaves of them, a second product, without which the error is 1.4 times that of rounding
 // the result.  Outputs are renewed only with a row's maximum, which follows its scores with some slack.
 //
-// The 8192 exponentials of a tile take 512 cycles of an SM at 16 a cycle; the products 256 with heads of 64.  Heads of up to 64 have two CTAs an
-// SM, so that one's waits and copies run under the other's softmax: 850 to 1000 cycles a tile and SM.  Eight sequences of 400 tokens over 1500,
-// 12 heads of 64 with 4 for keys: 48 us from 8-bit pages and 45 from bf16, 41 without the second product (8.2 GFLOP; by mma.sync, every warp converting all keys, 74 and 59),
-// of which 4 go into cutting the work and 8 into joining shared items; two of 100 over 60000, 16 heads of 128 with 2, 161 and 127 (334 by
+// The 8192 exponentials of a tile take 512 cycles of an SM at 16 a cycle; the products 256 with heads of 64, 384 over bf16 pages.  Heads of up to
+// 64 have two CTAs an SM, so that one's waits and copies run under the other's softmax: 850 to 1000 cycles a tile and SM.  Eight sequences of
+// 400 tokens over 1500, 12 heads of 64 with 4 for keys: 48 us from 8-bit pages and 45 from bf16, 41 without the second product (8.2 GFLOP; by
+// mma.sync, every warp converting all keys, 74 and 59).  Its 4452 tiles, 30 an SM, are about 15 of the 48; cutting the work is 4, joining shared
+// items 8, launches, starts and ends of items and what is uneven the rest.  Two of 100 over 60000, 16 heads of 128 with 2, 165 and 155 (334 by
 // mma.sync).  Two threads a row, with half of the keys each, took 60 and 49 in place of 52 and 45: registers for 22 warps are too few; half of the
-// scores loaded under the maximum of the others 50.4 and 42.6 in place of 49.2 and 41.6.
+// scores loaded under the maximum of the others 50.4 and 42.6 in place of 49.2 and 41.6 (bf16 without the second product, both).
 // Every wait is bounded and reports through the status word.
 #pragma once
 
@@ -37,7 +38,9 @@ struct Prompt {
   static constexpr int kMostSmem = 1024 + kQ + kStages * kStage + kRaws * kRaw;
   static constexpr int kInfo = 8;  // tiles whose scales and marks are kept
   static_assert(kLag + kStages < kInfo, "a tile's scales are written again when it is done with");
-  static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile, kRestart = 768 / kTile;
+  // as in Form; us at half, as is, and at twice as many.  alone: 8 x 400 over 200 35.0 20.3 20.3, over 500 39.2 39.2 25.2, 100 over 600 (bf16)
+  // 21.5 18.6 18.6; least: 8 x 100 over 1000 29.5 25.9 25.1, 50 over 3000 37.0 37.1 30.9
+  static constexpr int kAlone = 768 / kTile, kLeast = 256 / kTile;
 };
 
 // f16 or bf16 operands, 128 rows, n columns; values lie with their columns together
